@@ -1,0 +1,91 @@
+// Entry points of the attention operators: argument checks, and which kernels take a call.
+#include "attention.cuh"
+
+namespace lsr {
+namespace {
+
+constexpr int kMaxHeadDim = 128;
+
+bool dtype_ok(int d) { return d == LSR_DTYPE_F32 || d == LSR_DTYPE_BF16 || d == LSR_DTYPE_F16; }
+
+int check_args(const lsr_attention_args* a) {
+  if (!a || !dtype_ok(a->dtype)) return LSR_ERR_ARG;
+  if (a->batch < 0 || a->q_len < 0 || a->kv_len < 0 || a->heads < 1 || a->kv_heads < 1 || a->head_dim < 1) return LSR_ERR_ARG;
+  if (a->causal != 0 && a->causal != 1) return LSR_ERR_ARG;
+  if (a->heads % a->kv_heads || a->head_dim > kMaxHeadDim) return LSR_ERR_SHAPE;
+  // row numbers and block counts stay within 31 bits
+  if ((long long)a->batch * a->heads > (1ll << 24) || a->q_len > (1 << 30) || a->kv_len > (1 << 30)) return LSR_ERR_SHAPE;
+  return LSR_OK;
+}
+
+AttnStride stride_of(const long long* s) { return AttnStride{s[0], s[1], s[2]}; }
+
+AttnParams params_of(const lsr_attention_args* a) {
+  AttnParams p{};
+  p.batch = a->batch;
+  p.q_len = a->q_len;
+  p.kv_len = a->kv_len;
+  p.heads = a->heads;
+  p.kv_heads = a->kv_heads;
+  p.head_dim = a->head_dim;
+  p.causal = a->causal;
+  p.group = a->heads / a->kv_heads;
+  p.scale = a->scale;
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
+  p.out = a->out;
+  p.dout = a->dout;
+  p.dq = a->dq;
+  p.dk = a->dk;
+  p.dv = a->dv;
+  p.sq = stride_of(a->q_stride);
+  p.sk = stride_of(a->k_stride);
+  p.sv = stride_of(a->v_stride);
+  p.so = stride_of(a->out_stride);
+  p.sdo = stride_of(a->dout_stride);
+  p.sdq = stride_of(a->dq_stride);
+  p.sdk = stride_of(a->dk_stride);
+  p.sdv = stride_of(a->dv_stride);
+  p.mask = a->key_mask;
+  p.mask_stride = a->key_mask_stride;
+  p.lse = a->lse;
+  return p;
+}
+
+}  // namespace
+}  // namespace lsr
+
+extern "C" {
+
+size_t lsr_attention_backward_workspace_bytes(const lsr_attention_args* a) {
+  if (lsr::check_args(a) != LSR_OK) return 0;
+  return (size_t)a->batch * a->heads * a->q_len * sizeof(float) + 16;
+}
+
+int lsr_attention_forward(const lsr_attention_args* a, lsr_stream_t stream) {
+  using namespace lsr;
+  int rc = check_args(a);
+  if (rc != LSR_OK) return rc;
+  if (a->batch == 0 || a->q_len == 0) return LSR_OK;
+  if (!a->q || !a->out || !a->lse || (a->kv_len && (!a->k || !a->v))) return LSR_ERR_ARG;
+  if ((rc = check_device()) != LSR_OK) return rc;
+  AttnParams p = params_of(a);
+  return attention_forward_general(p, a->dtype, static_cast<cudaStream_t>(stream));
+}
+
+int lsr_attention_backward(const lsr_attention_args* a, void* ws, size_t ws_bytes, lsr_stream_t stream) {
+  using namespace lsr;
+  int rc = check_args(a);
+  if (rc != LSR_OK) return rc;
+  if (a->batch == 0 || (a->q_len == 0 && a->kv_len == 0)) return LSR_OK;
+  if (a->q_len && (!a->q || !a->dout || !a->out || !a->lse || !a->dq)) return LSR_ERR_ARG;
+  if (a->kv_len && (!a->k || !a->v || !a->dk || !a->dv)) return LSR_ERR_ARG;
+  if (!ws || ws_bytes < lsr_attention_backward_workspace_bytes(a)) return LSR_ERR_WORKSPACE;
+  if ((rc = check_device()) != LSR_OK) return rc;
+  AttnParams p = params_of(a);
+  p.delta = static_cast<float*>(ws);
+  return attention_backward_general(p, a->dtype, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -124,6 +124,13 @@ SIGNATURES: dict[str, tuple] = {
     "lsr_coupled_newton_f32": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_float, c_int,
                 c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "lsr_grad_workspace_bytes": (c_size_t, [c_int]),
+    "lsr_grad_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "lsr_grad_clip": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_int, c_void_p,
+                              c_void_p, c_size_t, c_void_p]),
+    "lsr_attention_backward_workspace_bytes": (c_size_t, [c_void_p]),
+    "lsr_attention_forward": (c_int, [c_void_p, c_void_p]),
+    "lsr_attention_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "lsr_ipc_alloc": (c_int, [c_size_t, ctypes.POINTER(c_void_p), c_void_p]),
     "lsr_ipc_open": (c_int, [c_void_p, ctypes.POINTER(c_void_p)]),
     "lsr_ipc_close": (c_int, [c_void_p]),

@@ -1,0 +1,178 @@
+"""Global gradient norm and clipping over every tensor of a model, in liblsr's kernels.
+
+* ``grad_norm(tensors, norm_type)``                   the norm of all tensors taken as one vector
+* ``clip_grads(grads, max_norm, norm_type, out, total_norm)``
+                                                      scaled by min(1, max_norm / (norm + 1e-6)), in
+                                                      place or into ``out`` of another type
+* ``clip_grad_norm_(parameters, max_norm, ...)``      the same on ``p.grad``, as
+                                                      ``torch.nn.utils.clip_grad_norm_`` is called
+
+The tensors may mix fp32, bf16 and fp16 and any shapes; norms are fp32 device scalars, summed in 64
+bits in one fixed order, and nothing waits for the device unless ``error_if_nonfinite`` is set. The
+list travels in the kernels' parameters, so a call can be captured into a CUDA graph. With gradients
+sharded over ranks: ``grad_norm`` on each rank's own, the ranks' norms combined (for norm 2 the root
+of the sum of squares), then ``clip_grads(..., total_norm=combined)``.
+
+The reference trains unclipped (muon_lm_ddp.py:1367-1381). There is no CPU path: CPU tensors raise
+``ValueError``.
+"""
+from __future__ import annotations
+
+import math
+from array import array
+
+import torch
+
+from . import _lib
+
+_KINDS = {math.inf: 0, 1.0: 1, 2.0: 2}
+
+
+def _kind(norm_type) -> int:
+    try:
+        return _KINDS[float(norm_type)]
+    except (KeyError, TypeError, ValueError):
+        raise ValueError(f"norm_type must be 1, 2 or inf (got {norm_type!r})") from None
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's entries fill one range of memory, each place once."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _check_list(tensors, what: str) -> list[torch.Tensor]:
+    ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    for t in ts:
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what} must be tensors")
+        if t.layout != torch.strided:
+            raise ValueError(f"{what} must be dense tensors (got {t.layout})")
+    for dtype, device in {(t.dtype, t.device) for t in ts}:
+        if device.type != "cuda":
+            raise ValueError(f"{what} must be CUDA tensors (liblsr has no CPU path)")
+        if dtype not in _lib.DTYPE_CODES:
+            raise ValueError(f"{what} must be fp32, bf16 or fp16 (got {dtype})")
+        if device != ts[0].device:
+            raise ValueError(f"{what} must be on one device (got {device} and {ts[0].device})")
+    return ts
+
+
+def _arrays(ts):
+    codes = _lib.DTYPE_CODES
+    return array("Q", [t.data_ptr() for t in ts]), array("i", [codes[t.dtype] for t in ts])
+
+
+def _workspace(lib, count: int, device: torch.device) -> torch.Tensor:
+    # of this call alone: calls on several streams, or graphs captured here, share nothing
+    return torch.empty(lib.lsr_grad_workspace_bytes(count), dtype=torch.uint8, device=device)
+
+
+def _address(a: array) -> int:
+    return a.buffer_info()[0]
+
+
+@torch.no_grad()
+def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm (1, 2 or inf) over every entry of every tensor: a 0-d fp32 tensor on their device."""
+    kind = _kind(norm_type)
+    ts = _check_list(tensors, "tensors")
+    if not ts:
+        return torch.zeros(())
+    ts = [t if _dense(t) else t.contiguous() for t in ts]
+    dev = ts[0].device
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ws = _workspace(lib, len(ts), dev)
+        ptrs, dtypes = _arrays(ts)
+        numel = array("q", [t.numel() for t in ts])
+        rc = lib.lsr_grad_norm(_address(ptrs), _address(numel), _address(dtypes), len(ts), kind, norm.data_ptr(),
+                               ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
+    _lib.check(rc, "lsr_grad_norm")
+    return norm
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_norm: torch.Tensor | None = None) -> torch.Tensor:
+    """Scale `grads` by min(1, max_norm / (norm + 1e-6)) and return the norm before it.
+
+    In place when `out` is None; else out[i] = grads[i] * coefficient in out[i]'s type (same shapes,
+    e.g. fp32 gradients to the bf16 that the Muon step takes), and out[i] may be grads[i] itself.
+    Apart from that no output may share memory with another output or with a gradient (ValueError).
+    `total_norm`: a 0-d fp32 device tensor to be used instead of computing the norm. A NaN norm makes
+    every entry NaN, an infinite one makes finite entries 0, as torch.nn.utils.clip_grad_norm_ does.
+    """
+    kind = _kind(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must be at least 0 (got {max_norm})")
+    ts = _check_list(grads, "grads")
+    outs = ts if out is None else _check_list(out, "out")
+    if len(outs) != len(ts) or any(o.shape != t.shape for o, t in zip(outs, ts)):
+        raise ValueError("out must be one tensor of the same shape for each gradient")
+    if not ts:
+        return torch.zeros(()) if total_norm is None else total_norm
+    dev = ts[0].device
+    if outs[0].device != dev:
+        raise ValueError("out must be on the gradients' device")
+    if total_norm is not None and (total_norm.dtype != torch.float32 or total_norm.device != dev or total_norm.numel() != 1):
+        raise ValueError("total_norm must be one fp32 value on the gradients' device")
+    back = []  # (output, dense tensor to copy into it)
+    src, dst = [], []
+    for t, o in zip(ts, outs):
+        if t.is_contiguous() and o.is_contiguous():
+            src.append(t)
+            dst.append(o)
+        elif _dense(t) and _dense(o) and t.stride() == o.stride():
+            src.append(t)
+            dst.append(o)
+        else:
+            if any(st == 0 and sz > 1 for st, sz in zip(o.stride(), o.shape)):
+                raise ValueError("an output's entries share memory (an expanded tensor): clip a copy of it")
+            src.append(t.contiguous())
+            dst.append(o if o.is_contiguous() and o is not t else torch.empty(o.shape, dtype=o.dtype, device=dev))
+            if dst[-1] is not o:
+                back.append((o, dst[-1]))
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev) if total_norm is None else total_norm
+        ws = _workspace(lib, len(src), dev) if total_norm is None else None
+        pin, tin = _arrays(src)
+        pout, tout = _arrays(dst)
+        numel = array("q", [t.numel() for t in src])
+        rc = lib.lsr_grad_clip(_address(pin), _address(pout), _address(numel), _address(tin), _address(tout), len(src),
+                               kind, max_norm, int(total_norm is not None), norm.data_ptr(),
+                               ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                               _lib.stream_handle(dev))
+        _lib.check(rc, "lsr_grad_clip")
+        for o, t in back:
+            o.copy_(t)
+    return norm
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Clip the gradients of `parameters` in place by their global norm and return it (0-d fp32).
+
+    Parameters without a gradient are passed over; one listed twice counts once. With
+    `error_if_nonfinite` the norm is read back first, and a NaN or infinite one raises RuntimeError
+    with the gradients as they were.
+    """
+    ps = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads = list({id(p): p.grad for p in ps if p.grad is not None}.values())
+    if not error_if_nonfinite:
+        return clip_grads(grads, max_norm, norm_type)
+    norm = grad_norm(grads, norm_type)
+    if not math.isfinite(float(norm)):
+        raise RuntimeError(f"the gradients' norm of order {float(norm_type)} is {float(norm)}: they are not clipped")
+    return clip_grads(grads, max_norm, norm_type, total_norm=norm) if grads else norm
+
+
+__all__ = ["grad_norm", "clip_grads", "clip_grad_norm_"]

@@ -20,6 +20,11 @@ is recorded in the summary's extra ``"lsr"`` entry:
 * the token stream comes from ``--train-token-cache`` when that file exists (the reference's
   cache format, a 1-D token tensor); otherwise it is seeded synthetic tokens, uniform over the
   vocabulary, with the cache's length, and the summary says so.
+* ``--max-grad-norm X`` clips the gradients by their global norm before the optimizer
+  (``lsr.clip_grad_norm_``; 0, the default, leaves them);
+* ``--attention lsr`` runs the model's attention, forward and backward, in liblsr's kernels
+  (``lsr.attention``) instead of the model library's; they have no dropout, so that the model
+  needs ``--config-overrides attn_pdrop=0``;
 * ``--config-overrides key=value,...`` changes fields of the model configuration (small
   models for tests).
 """
@@ -79,6 +84,10 @@ def build_parser() -> argparse.ArgumentParser:
     # additions (not in the reference)
     p.add_argument("--muon-sharded", action="store_true",
                    help="shard the Muon matrices over the ranks (ZeRO-1) instead of replicating the step")
+    p.add_argument("--max-grad-norm", type=float, default=0.0,
+                   help="clip the gradients by their global norm (0: not)")
+    p.add_argument("--attention", choices=["model", "lsr"], default="model",
+                   help="whose attention kernels the model runs")
     p.add_argument("--config-overrides", type=str, default="",
                    help="comma-separated key=value changes to the model configuration")
     return p
@@ -101,17 +110,49 @@ def model_config(model_id: str, overrides: str):
     return cfg
 
 
+def _lsr_attention_mask(*, mask_function=None, attention_mask=None, **_):
+    """What lsr.attention takes of a mask: the padding, bool [batch, kv_len] or None; causality is a flag."""
+    if getattr(mask_function, "__name__", "") != "causal_mask_function":
+        raise ValueError("--attention lsr: the model asks for a mask other than causal and padding")
+    return attention_mask
+
+
+def _lsr_attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, is_causal=None, **kw):
+    """lsr.attention as the transformers library calls an attention function ([batch, heads, length, dim])."""
+    from .attention import attention
+    if dropout:
+        raise ValueError(f"--attention lsr has no dropout (the model's is {dropout}): "
+                         "use --config-overrides attn_pdrop=0")
+    for name in ("sliding_window", "softcap", "s_aux", "position_bias", "head_mask"):
+        if kw.get(name) is not None:
+            raise ValueError(f"--attention lsr: the model passes {name}")
+    if is_causal is None:
+        is_causal = getattr(module, "is_causal", True)
+    mask = None if attention_mask is None else attention_mask.bool()
+    out = attention(query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2), causal=bool(is_causal),
+                    scale=scaling, key_mask=mask)
+    return out, None
+
+
+def _register_attention() -> str:
+    from transformers import AttentionInterface, AttentionMaskInterface
+    AttentionInterface.register("lsr", _lsr_attention)
+    AttentionMaskInterface.register("lsr", _lsr_attention_mask)
+    return "lsr"
+
+
 def load_model(args, device):
     """The model as muon_lm_ddp.load_model_and_tokenizer builds it (:755-826): bf16, use_cache off,
     optional gradient checkpointing, train mode."""
     from transformers import AutoModelForCausalLM
+    attn = {"attn_implementation": _register_attention()} if args.attention == "lsr" else {}
     if args.init == "pretrained":
         if not Path(args.model_id).is_dir():
             raise RuntimeError("--init pretrained needs a local model directory as --model-id "
                                "(no download here); use --init random for the random-init benchmark")
-        model = AutoModelForCausalLM.from_pretrained(args.model_id, dtype=torch.bfloat16)
+        model = AutoModelForCausalLM.from_pretrained(args.model_id, dtype=torch.bfloat16, **attn)
     else:
-        model = AutoModelForCausalLM.from_config(model_config(args.model_id, args.config_overrides))
+        model = AutoModelForCausalLM.from_config(model_config(args.model_id, args.config_overrides), **attn)
         model = model.to(dtype=torch.bfloat16)
     model.config.use_cache = False
     if args.gradient_checkpointing:
@@ -182,6 +223,9 @@ class _ShardedMuonAdamW:
     def adam_step(self):
         self.base.adam_step()
 
+    def clip_grad_norm(self, max_norm):
+        return self.base.clip_grad_norm(max_norm)
+
     def zero_grad(self):
         self.base.zero_grad()
 
@@ -250,6 +294,7 @@ def main(argv=None) -> int:
                     loss = ddp_model(input_ids=x, labels=x, use_cache=False).loss / args.grad_accum
                 loss.backward()
             total_loss += float(loss.detach())
+        grad_norm = optimizer.clip_grad_norm(args.max_grad_norm) if args.max_grad_norm > 0 else None
         ev[1].record()
         optimizer.muon_step()
         ev[2].record()
@@ -272,7 +317,8 @@ def main(argv=None) -> int:
         if rank == 0 and (step % args.log_every == 0 or step == args.steps - 1):
             print(f"[{'MEASURE' if measured else 'WARMUP'}] step={step:03d} loss={loss_mean:.5f} "
                   f"step={step_ms:.1f}ms opt={opt_ms:.1f}ms muon={muon_ms:.1f}ms adam={adam_ms:.1f}ms "
-                  f"tok/s={global_tokens_per_step / (step_ms / 1000.0):,.0f}", flush=True)
+                  f"tok/s={global_tokens_per_step / (step_ms / 1000.0):,.0f}"
+                  + (f" grad_norm={float(grad_norm):.4f}" if grad_norm is not None else ""), flush=True)
     if not step_ms_values:
         raise RuntimeError("No measured steps. Set --steps > --warmup-steps.")
     peak_gb = _max(torch.cuda.max_memory_allocated(device) / 1024 ** 3, device, world)
@@ -305,7 +351,8 @@ def main(argv=None) -> int:
         "optimizer_structure": opt_summary,
         "lsr": {"optimizer": "lsr.MuonAdamW" + (" + lsr.dist.ShardedMuon" if args.muon_sharded and world > 1
                                                  else ""),
-                "data": data_source, "config_overrides": args.config_overrides},
+                "data": data_source, "config_overrides": args.config_overrides,
+                "attention": args.attention, "max_grad_norm": args.max_grad_norm},
     }
     if rank == 0:
         for key in ("median_step_ms", "median_optimizer_ms", "median_muon_ms", "median_adam_ms",

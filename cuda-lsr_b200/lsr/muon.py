@@ -21,6 +21,7 @@ from collections import defaultdict
 import torch
 
 from . import _lib
+from .grad import clip_grad_norm_
 
 NS_A = 3.4445
 NS_B = -4.7750
@@ -303,6 +304,12 @@ class MuonAdamW:
             p.grad = None
         if self.adam is not None:
             self.adam.zero_grad(set_to_none=True)
+
+    def clip_grad_norm(self, max_norm, norm_type=2.0, error_if_nonfinite=False):
+        """Clip the gradients of every Muon and AdamW parameter in place by their global norm; call it
+        between the backward pass and the steps. Returns the norm (lsr.grad.clip_grad_norm_)."""
+        return clip_grad_norm_([p for _, p in self.muon_named + self.adam_named], max_norm, norm_type,
+                               error_if_nonfinite)
 
     def _items(self):
         items = []

@@ -45,7 +45,7 @@ typedef struct CUstream_st* lsr_stream_t; /* == cudaStream_t */
 #define LSR_ERR_TOO_LARGE (-7) /* problem exceeds the fixed scratch capacity */
 #define LSR_ERR_PEER (-8)      /* CUDA IPC / peer memory call failed         */
 
-/* Element types of lsr_blocks_apply_any's update operand. */
+/* Element types (of lsr_blocks_apply_any's update operand, of gradients, of attention). */
 #define LSR_DTYPE_F32 0
 #define LSR_DTYPE_BF16 1
 #define LSR_DTYPE_F16 2
@@ -432,6 +432,70 @@ LSR_API size_t lsr_coupled_newton_workspace_bytes(int batch, int n);
 LSR_API int lsr_coupled_newton_f32(const float* A, float* X, int* iters, float* err, int* redo, int batch, int n,
                                    int root, float epsilon, float tolerance, int max_iterations, int check_every,
                                    int use_tf32, void* ws, size_t ws_bytes, lsr_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Global gradient norm and clipping. New: the reference trains unclipped
+ * (muon_lm_ddp.py:1367-1381 goes from the backward pass to the optimizer).
+ *
+ * `count` tensors given by host arrays: device pointers, entry counts and
+ * element types (LSR_DTYPE_*); tensors of no entries are skipped. The arrays
+ * are read before the call returns. norm_kind: 0 the largest |g|, 1 the sum
+ * of |g|, 2 the square root of the sum of squares. Sums are held in 64 bits
+ * and added in one fixed order.
+ * lsr_grad_norm: *norm (device, fp32) = the norm over every entry.
+ * lsr_grad_clip: outs[i] = round(grads[i] * min(1, max_norm / (norm + 1e-6))).
+ *   outs[i] may be grads[i] with the same type (in place); otherwise no output
+ *   may overlap another output or any input (LSR_ERR_ARG). norm_given = 0: *norm
+ *   is computed over these tensors and written; 1: *norm is read (the norm of
+ *   more tensors than these, e.g. over all ranks) and ws may be NULL. A NaN
+ *   norm makes every output NaN, an infinite one makes finite entries zero.
+ * ---------------------------------------------------------------------- */
+LSR_API size_t lsr_grad_workspace_bytes(int count);
+LSR_API int lsr_grad_norm(const void* const* grads, const long long* numel, const int* dtypes, int count, int norm_kind,
+                          float* norm, void* ws, size_t ws_bytes, lsr_stream_t stream);
+LSR_API int lsr_grad_clip(const void* const* grads, void* const* outs, const long long* numel, const int* dtypes,
+                          const int* out_dtypes, int count, int norm_kind, float max_norm, int norm_given,
+                          float* norm, void* ws, size_t ws_bytes, lsr_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Softmax attention with its log-sum-exp, and its gradients. New: the
+ * reference's models leave attention to their model library.
+ *
+ *   s_ij = scale q_i . k_j, minus infinity where query i does not see key j
+ *   lse_i = log sum_j exp s_ij,  p_ij = exp(s_ij - lse_i),  out_i = sum_j p_ij v_j
+ *   ds_ij = scale p_ij (dout_i . v_j - dout_i . out_i)
+ *   dv_j = sum_i p_ij dout_i,  dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i
+ * A query that sees no key: out 0, lse minus infinity, no gradient.
+ * Query head h reads key head h / (heads / kv_heads); dk and dv sum over the
+ * query heads of a key head. causal: query i sees keys j <= i + kv_len - q_len
+ * (the last query sees the last key). key_mask [batch][kv_len] bytes, rows
+ * key_mask_stride apart, nonzero = seen, may be NULL; what a masked key's rows
+ * of k and v hold does not matter, NaN included. head_dim 1..128; strides in
+ * elements (batch, position, head), the head_dim entries of a head contiguous.
+ * Probabilities and sums are fp32; with 16-bit types p and ds are rounded to
+ * that type as operands of the products that take them.
+ * lsr_attention_forward reads q, k, v, key_mask and writes out and lse
+ * (fp32 [batch][heads][q_len]); lsr_attention_backward reads those, dout and
+ * what the forward pass wrote, and writes dq, dk, dv. No atomics: the same
+ * inputs give the same bits.
+ * ---------------------------------------------------------------------- */
+typedef struct lsr_attention_args {
+  int dtype; /* LSR_DTYPE_* of every tensor but lse */
+  int batch, q_len, kv_len, heads, kv_heads, head_dim, causal;
+  float scale;
+  const void *q, *k, *v;
+  const unsigned char* key_mask;
+  void* out;
+  float* lse;
+  const void* dout;
+  void *dq, *dk, *dv;
+  long long q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3],
+      dv_stride[3];
+  long long key_mask_stride;
+} lsr_attention_args;
+LSR_API size_t lsr_attention_backward_workspace_bytes(const lsr_attention_args* args);
+LSR_API int lsr_attention_forward(const lsr_attention_args* args, lsr_stream_t stream);
+LSR_API int lsr_attention_backward(const lsr_attention_args* args, void* ws, size_t ws_bytes, lsr_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Peer-memory exchange of finished parameter shards (sharded Muon step).
