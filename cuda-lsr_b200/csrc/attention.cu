@@ -1,5 +1,5 @@
 // Entry points of the attention operators: argument checks, and which kernels take a call.
-#include "attention.cuh"
+#include "attention_sm100.cuh"
 
 namespace lsr {
 namespace {
@@ -53,17 +53,34 @@ AttnParams params_of(const lsr_attention_args* a) {
   return p;
 }
 
+// The tensor-core kernels read by TMA: 16-bit types, 16-byte addresses, strides and rows. They take the
+// row maximum of unscaled scores, which is that of the scaled ones for a positive scale.
+bool fast_forward(const AttnParams& p, int dtype) {
+  return dtype != LSR_DTYPE_F32 && p.scale > 0.f && p.kv_len > 0 && (!p.mask || p.kv_len <= kMaskTiles * kRows) &&
+         rows_ok(p.q, p.sq, p.batch, p.heads, p.q_len, p.head_dim) &&
+         rows_ok(p.k, p.sk, p.batch, p.kv_heads, p.kv_len, p.head_dim) &&
+         rows_ok(p.v, p.sv, p.batch, p.kv_heads, p.kv_len, p.head_dim) &&
+         rows_ok(p.out, p.so, p.batch, p.heads, p.q_len, p.head_dim);
+}
+
 }  // namespace
 }  // namespace lsr
 
 extern "C" {
+
+size_t lsr_attention_forward_workspace_bytes(const lsr_attention_args* a) {
+  using namespace lsr;
+  if (check_args(a) != LSR_OK || a->batch == 0 || a->q_len == 0) return 0;
+  const AttnParams p = params_of(a);
+  return fast_forward(p, a->dtype) ? attention_forward_sm100_ws(p) : 0;
+}
 
 size_t lsr_attention_backward_workspace_bytes(const lsr_attention_args* a) {
   if (lsr::check_args(a) != LSR_OK) return 0;
   return (size_t)a->batch * a->heads * a->q_len * sizeof(float) + 16;
 }
 
-int lsr_attention_forward(const lsr_attention_args* a, lsr_stream_t stream) {
+int lsr_attention_forward(const lsr_attention_args* a, void* ws, size_t ws_bytes, lsr_stream_t stream) {
   using namespace lsr;
   int rc = check_args(a);
   if (rc != LSR_OK) return rc;
@@ -71,7 +88,11 @@ int lsr_attention_forward(const lsr_attention_args* a, lsr_stream_t stream) {
   if (!a->q || !a->out || !a->lse || (a->kv_len && (!a->k || !a->v))) return LSR_ERR_ARG;
   if ((rc = check_device()) != LSR_OK) return rc;
   AttnParams p = params_of(a);
-  return attention_forward_general(p, a->dtype, static_cast<cudaStream_t>(stream));
+  if (!fast_forward(p, a->dtype)) return attention_forward_general(p, a->dtype, static_cast<cudaStream_t>(stream));
+  const size_t need = attention_forward_sm100_ws(p);
+  if (need && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15))) return LSR_ERR_WORKSPACE;
+  if (!(p.status = status_ptr())) return LSR_ERR_LAUNCH;
+  return attention_forward_sm100(p, a->dtype, ws, static_cast<cudaStream_t>(stream));
 }
 
 int lsr_attention_backward(const lsr_attention_args* a, void* ws, size_t ws_bytes, lsr_stream_t stream) {

@@ -193,6 +193,18 @@ int encode_tmap_mn_chunks(CUtensorMap* map, CUtensorMapDataType dtype, int elem_
   return r == CUDA_SUCCESS ? LSR_OK : LSR_ERR_DRIVER;
 }
 
+int encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[4],
+                   const uint64_t (&strides)[3], const uint32_t (&box)[4]) {
+  EncodeTiledFn encode = encode_fn();
+  if (!encode) return LSR_ERR_DRIVER;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || ((strides[0] | strides[1] | strides[2]) & 15)) return LSR_ERR_SHAPE;
+  cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, st[3] = {strides[0], strides[1], strides[2]};
+  cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]}, estr[4] = {1, 1, 1, 1};
+  CUresult r = encode(map, dtype, 4, const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? LSR_OK : LSR_ERR_DRIVER;
+}
+
 int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, int elem_bytes, const void* base, uint64_t inner,
                    uint64_t outer, uint64_t batch, uint64_t ld, uint64_t bstride, uint32_t box_inner,
                    uint32_t box_outer, CUtensorMapSwizzle swizzle) {

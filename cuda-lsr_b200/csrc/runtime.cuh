@@ -26,6 +26,10 @@ int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, int elem_bytes, 
                    uint64_t outer, uint64_t batch, uint64_t ld, uint64_t bstride, uint32_t box_inner,
                    uint32_t box_outer, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
+// Encode a 4-D tensor map, dims[0] contiguous, strides in bytes, 128-byte swizzle.
+int encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[4],
+                   const uint64_t (&strides)[3], const uint32_t (&box)[4]);
+
 // Launch accounting / optional per-launch timing. Kinds group the library's
 // kernels for the profile read-out (lsr_profile_read).
 enum ProfKind : int {

@@ -129,7 +129,8 @@ SIGNATURES: dict[str, tuple] = {
     "lsr_grad_clip": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_int, c_void_p,
                               c_void_p, c_size_t, c_void_p]),
     "lsr_attention_backward_workspace_bytes": (c_size_t, [c_void_p]),
-    "lsr_attention_forward": (c_int, [c_void_p, c_void_p]),
+    "lsr_attention_forward_workspace_bytes": (c_size_t, [c_void_p]),
+    "lsr_attention_forward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "lsr_attention_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "lsr_ipc_alloc": (c_int, [c_size_t, ctypes.POINTER(c_void_p), c_void_p]),
     "lsr_ipc_open": (c_int, [c_void_p, ctypes.POINTER(c_void_p)]),

@@ -81,6 +81,11 @@ def _pack(q, k, v, key_mask, causal, scale, out, lse, dout=None, dq=None, dk=Non
                       key_mask.stride(0) if key_mask is not None else 0)
 
 
+def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
+    # of this call alone: calls on several streams, or graphs captured here, share nothing
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _scale(scale, q) -> float:
     return float(q.shape[3]) ** -0.5 if scale is None else float(scale)
 
@@ -95,8 +100,10 @@ def attention_forward(q, k, v, *, causal: bool = False, scale: float | None = No
     with _lib.on_device(q.device):
         out = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
         lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device)
-        rc = lib.lsr_attention_forward(_pack(q, k, v, key_mask, causal, _scale(scale, q), out, lse),
-                                       _lib.stream_handle(q.device))
+        args = _pack(q, k, v, key_mask, causal, _scale(scale, q), out, lse)
+        nbytes = lib.lsr_attention_forward_workspace_bytes(args)
+        ws = _workspace(nbytes, q.device)
+        rc = lib.lsr_attention_forward(args, ws.data_ptr() if nbytes else None, nbytes, _lib.stream_handle(q.device))
     _lib.check(rc, "lsr_attention_forward")
     return out, lse
 
@@ -117,8 +124,7 @@ def attention_backward(dout, q, k, v, out, lse, *, causal: bool = False, scale: 
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         args = _pack(q, k, v, key_mask, causal, _scale(scale, q), out, lse, dout, dq, dk, dv)
         nbytes = lib.lsr_attention_backward_workspace_bytes(args)
-        # of this call alone: calls on several streams, or graphs captured here, share nothing
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws = _workspace(nbytes, q.device)
         rc = lib.lsr_attention_backward(args, ws.data_ptr(), nbytes, _lib.stream_handle(q.device))
     _lib.check(rc, "lsr_attention_backward")
     return dq, dk, dv

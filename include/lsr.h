@@ -8,7 +8,7 @@
  *   - nothing allocates: scratch memory comes from the caller's workspace
  *     (`ws`, `ws_bytes`), sized by the matching *_workspace_bytes() query;
  *   - the return value is LSR_OK or a negative LSR_ERR_* code; device-side
- *     failures (a bounded wait that timed out: codes 101-107; an event index
+ *     failures (a bounded wait that timed out: codes 101-107, 120-123; an event index
  *     out of range: 110) are recorded in the library's device status word,
  *     read with lsr_device_status();
  *   - calls are thread-safe as long as concurrent calls use distinct
@@ -477,7 +477,10 @@ LSR_API int lsr_grad_clip(const void* const* grads, void* const* outs, const lon
  * lsr_attention_forward reads q, k, v, key_mask and writes out and lse
  * (fp32 [batch][heads][q_len]); lsr_attention_backward reads those, dout and
  * what the forward pass wrote, and writes dq, dk, dv. No atomics: the same
- * inputs give the same bits.
+ * inputs give the same bits. Workspaces are 16-byte aligned; a size of 0 needs
+ * none. 16-bit tensors whose addresses, strides and rows are multiples of 16
+ * bytes, with a positive scale, run on the tensor cores; all others in fp32
+ * on the CUDA cores.
  * ---------------------------------------------------------------------- */
 typedef struct lsr_attention_args {
   int dtype; /* LSR_DTYPE_* of every tensor but lse */
@@ -493,8 +496,9 @@ typedef struct lsr_attention_args {
       dv_stride[3];
   long long key_mask_stride;
 } lsr_attention_args;
+LSR_API size_t lsr_attention_forward_workspace_bytes(const lsr_attention_args* args);
+LSR_API int lsr_attention_forward(const lsr_attention_args* args, void* ws, size_t ws_bytes, lsr_stream_t stream);
 LSR_API size_t lsr_attention_backward_workspace_bytes(const lsr_attention_args* args);
-LSR_API int lsr_attention_forward(const lsr_attention_args* args, lsr_stream_t stream);
 LSR_API int lsr_attention_backward(const lsr_attention_args* args, void* ws, size_t ws_bytes, lsr_stream_t stream);
 
 /* ------------------------------------------------------------------------

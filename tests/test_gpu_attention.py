@@ -112,6 +112,18 @@ def test_shapes_and_types(shape, dtype, causal):
     Case(*tensors(*shape, dtype, seed=sum(shape)), causal=causal)
 
 
+@pytest.mark.parametrize("n,m,d,kv,causal,masked", [
+    (400, 400, 64, 40, True, False), (260, 300, 128, 8, False, False), (300, 600, 64, 20, True, True),
+    (600, 300, 128, 40, True, False), (257, 140, 80, 8, False, True)])
+def test_many_heads(n, m, d, kv, causal, masked):
+    """Enough blocks for every SM, lengths that end inside a tile and inside a pair of tiles."""
+    q, k, v, do = tensors(2, n, m, 40, kv, d, torch.bfloat16, seed=n + d)
+    mask = None
+    if masked:
+        mask = torch.arange(m, device="cuda") < torch.tensor([[m - 3], [m // 2]], device="cuda")
+    Case(q, k, v, do, causal=causal, key_mask=mask)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("kind", ["right", "left", "holes", "empty entry", "one key", "far tiles"])

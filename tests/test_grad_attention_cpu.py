@@ -58,14 +58,15 @@ def test_attention_c_abi_rejects_bad_arguments_before_any_device_work():
     lib = _lib.load()
     size = lib.lsr_attention_backward_workspace_bytes
     assert size(_args()) >= 2 * 6 * 3 * 4
-    assert lib.lsr_attention_forward(None, None) == -1
+    assert lib.lsr_attention_forward(None, None, 0, None) == -1
     for bad, rc in ((dict(dtype=3), -1), (dict(b=-1), -1), (dict(h=0), -1), (dict(d=0), -1), (dict(causal=2), -1),
                     (dict(hk=4), -2), (dict(d=129), -2), (dict(b=1 << 24), -2)):
-        assert lib.lsr_attention_forward(_args(**bad), None) == rc, bad
+        assert lib.lsr_attention_forward(_args(**bad), None, 0, None) == rc, bad
         assert lib.lsr_attention_backward(_args(**bad), 4096, 1 << 20, None) == rc, bad
         assert size(_args(**bad)) == 0
     assert lib.lsr_attention_backward(_args(), 4096, 16, None) == -3
-    assert lib.lsr_attention_forward(_args(b=0), None) == 0 and lib.lsr_attention_forward(_args(n=0), None) == 0
+    assert lib.lsr_attention_forward(_args(b=0), None, 0, None) == 0
+    assert lib.lsr_attention_forward(_args(n=0), None, 0, None) == 0
 
 
 def test_cpu_tensors_are_refused():
