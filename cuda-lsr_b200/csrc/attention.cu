@@ -63,6 +63,13 @@ bool fast_forward(const AttnParams& p, int dtype) {
          rows_ok(p.out, p.so, p.batch, p.heads, p.q_len, p.head_dim);
 }
 
+bool fast_backward(const AttnParams& p, int dtype) {
+  return p.q_len > 0 && fast_forward(p, dtype) && rows_ok(p.dout, p.sdo, p.batch, p.heads, p.q_len, p.head_dim) &&
+         rows_ok(p.dq, p.sdq, p.batch, p.heads, p.q_len, p.head_dim) &&
+         rows_ok(p.dk, p.sdk, p.batch, p.kv_heads, p.kv_len, p.head_dim) &&
+         rows_ok(p.dv, p.sdv, p.batch, p.kv_heads, p.kv_len, p.head_dim);
+}
+
 }  // namespace
 }  // namespace lsr
 
@@ -76,7 +83,10 @@ size_t lsr_attention_forward_workspace_bytes(const lsr_attention_args* a) {
 }
 
 size_t lsr_attention_backward_workspace_bytes(const lsr_attention_args* a) {
-  if (lsr::check_args(a) != LSR_OK) return 0;
+  using namespace lsr;
+  if (check_args(a) != LSR_OK || a->batch == 0) return 0;
+  const AttnParams p = params_of(a);
+  if (fast_backward(p, a->dtype)) return attention_backward_sm100_ws(p);
   return (size_t)a->batch * a->heads * a->q_len * sizeof(float) + 16;
 }
 
@@ -102,9 +112,14 @@ int lsr_attention_backward(const lsr_attention_args* a, void* ws, size_t ws_byte
   if (a->batch == 0 || (a->q_len == 0 && a->kv_len == 0)) return LSR_OK;
   if (a->q_len && (!a->q || !a->dout || !a->out || !a->lse || !a->dq)) return LSR_ERR_ARG;
   if (a->kv_len && (!a->k || !a->v || !a->dk || !a->dv)) return LSR_ERR_ARG;
-  if (!ws || ws_bytes < lsr_attention_backward_workspace_bytes(a)) return LSR_ERR_WORKSPACE;
+  if (!ws || ws_bytes < lsr_attention_backward_workspace_bytes(a) || (reinterpret_cast<uintptr_t>(ws) & 15))
+    return LSR_ERR_WORKSPACE;
   if ((rc = check_device()) != LSR_OK) return rc;
   AttnParams p = params_of(a);
+  if (fast_backward(p, a->dtype)) {
+    if (!(p.status = status_ptr())) return LSR_ERR_LAUNCH;
+    return attention_backward_sm100(p, a->dtype, ws, static_cast<cudaStream_t>(stream));
+  }
   p.delta = static_cast<float*>(ws);
   return attention_backward_general(p, a->dtype, static_cast<cudaStream_t>(stream));
 }

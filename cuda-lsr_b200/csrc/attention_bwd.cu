@@ -1,0 +1,466 @@
+// Softmax attention's gradients on the tensor cores, 16-bit types.
+//
+//   P = exp2(S c - lse log2 e),  S = Q K^T,  c = scale log2 e;   dP = dO V^T,  D = rowsum(dO o O)
+//   dS = P o (dP - D);   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K
+//
+// A first kernel takes D and lse log2 e per row. One launch then runs two kinds of blocks. A key block
+// keeps 128 keys of one key head and passes over the queries that see them, of all the heads that share
+// the key head: it computes S^T = K Q^T and dP^T = V dO^T, a thread per key and half of the queries, and
+// adds P^T dO and dS^T Q in TMEM. A query block keeps 128 queries and passes over the keys: S, dP and
+// dS K. So S and dP are computed twice (7 products where 5 would do), and in return dK, dV and dQ are
+// each summed by one block in one order: no atomics, no second pass over a 32-bit dQ in memory, and
+// the gradients of a shared key head need no reduction.
+// Both kinds run the same pipeline. Per step, T1 = S (or S^T) and T2 = dP (or dP^T) lie in TMEM; P
+// overwrites T1 and dS overwrites T2 as 16-bit operands. The products of one step and the scores of the
+// next are issued as their operands get ready: while the threads take the exponentials of T1, the
+// tensor core adds dS and computes the next T2; while they form dS, it adds P and computes the next T1.
+// P and dS are rounded to 16 bits for the products. In fp16 P is taken times 2^10 (at most 1024), so
+// that rows over thousands of keys stay above its smallest normal value; dV is scaled back.
+#include "attention_sm100.cuh"
+
+namespace lsr {
+namespace {
+
+constexpr int BWD_THREADS = 384;  // two warpgroups on the scores, then the loader, the issuer and two idle warps
+constexpr int LOADER = 8, ISSUER = 9;
+
+// Extra power of two in P.
+template <typename T>
+constexpr int kExtra = 0;
+template <>
+constexpr int kExtra<__half> = 10;
+
+struct BwdParams {
+  AttnParams a;
+  CUtensorMap mq, mk, mv, mdo;
+  float* stats;  // [batch][heads][query tiles][2][128]: lse log2 e - extra (plus infinity: no probability), D 2^-extra
+  int q_tiles, kv_tiles;
+  long long kv_blocks;
+};
+
+template <int PANELS, bool MASK>
+struct BwdSmem {
+  static constexpr int TILE = PANELS * kPanel;
+  static constexpr int STAGES = PANELS == 1 ? 8 : 4;  // tiles in the ring, two per step
+  static constexpr int STATS = (2 + STAGES) * TILE;   // 1 KB per step in the ring
+  static constexpr int BITS = STATS + STAGES / 2 * 1024;
+  static constexpr int BARS = BITS + (MASK ? kMaskTiles * 16 : 0);
+  static constexpr int TOTAL = BARS + 256 + 1024;  // and room to align the tiles
+};
+
+// Row statistics, eight lanes per row.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ BwdParams p) {
+  const long long row = (long long)blockIdx.x * 32 + threadIdx.x / 8;  // rows of whole tiles
+  const int len = p.q_tiles * kRows, part = threadIdx.x % 8;
+  const int i = (int)(row % len), h = (int)(row / len % p.a.heads), b = (int)(row / len / p.a.heads);
+  if (b >= p.a.batch) return;
+  float s = 0.f, lse = INFINITY;
+  if (i < p.a.q_len) {
+    const T* o = attn_at<T>(p.a.out, p.a.so, b, h) + i * p.a.so.s;
+    const T* d = attn_at<T>(p.a.dout, p.a.sdo, b, h) + i * p.a.sdo.s;
+    for (int e = part * 8; e < p.a.head_dim; e += 64) {
+      const uint4 x = *reinterpret_cast<const uint4*>(o + e), y = *reinterpret_cast<const uint4*>(d + e);
+      const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s = fmaf(attn_to_f(xe[k]), attn_to_f(ye[k]), s);
+    }
+    const float v = p.a.lse[((long long)b * p.a.heads + h) * p.a.q_len + i];
+    if (v != -INFINITY) lse = fmaf(v, kLog2e, -(float)kExtra<T>);
+  }
+#pragma unroll
+  for (int w = 4; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+  if (part == 0) {
+    float* dst = p.stats + row / kRows * 256 + row % kRows;
+    dst[0] = lse;
+    dst[128] = s * (1.f / (1 << kExtra<T>));
+  }
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// Rows of an accumulator (32 columns at a time) to [position][entry], times `mul`; zeros where !any.
+template <typename T>
+__device__ __forceinline__ void store_rows(T* dst, uint32_t at, int col0, int col1, int dim, bool live, bool any, float mul) {
+  for (int q = col0; q < col1; q += 32) {
+    uint32_t o[32];
+    tmem_ld32(at + q, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; e += 8)
+      if (live && q + e < dim) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (any) {
+          v.x = pack2<T>(__uint_as_float(o[e]) * mul, __uint_as_float(o[e + 1]) * mul);
+          v.y = pack2<T>(__uint_as_float(o[e + 2]) * mul, __uint_as_float(o[e + 3]) * mul);
+          v.z = pack2<T>(__uint_as_float(o[e + 4]) * mul, __uint_as_float(o[e + 5]) * mul);
+          v.w = pack2<T>(__uint_as_float(o[e + 6]) * mul, __uint_as_float(o[e + 7]) * mul);
+        }
+        *reinterpret_cast<uint4*>(dst + q + e) = v;
+      }
+  }
+}
+
+template <typename T, int PANELS, bool MASK, bool KEYS>
+__device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_t* smem) {
+  using L = BwdSmem<PANELS, MASK>;
+  constexpr int STAGES = L::STAGES;
+  uint8_t *r1 = smem, *r2 = smem + L::TILE, *ring = smem + 2 * L::TILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
+  uint64_t *fixed = bars, *full = fixed + 1, *empty = full + STAGES, *t1_full = empty + STAGES, *t2_full = t1_full + 1,
+           *p_ready = t2_full + 1, *ds_ready = p_ready + 1, *done = ds_ready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int off = p.a.kv_len - p.a.q_len;  // under causality query i sees keys up to i + off
+  int* status = p.a.status;
+
+  // the block's rows, and the tiles of the other side that it passes over
+  int tile, h, b, first = 0, tiles;
+  if (KEYS) {
+    tile = (int)(x % p.kv_tiles);  // under causality the first keys are seen by the most queries
+    x /= p.kv_tiles;
+    h = (int)(x % p.a.kv_heads);
+    b = (int)(x / p.a.kv_heads);
+    if (p.a.causal) first = min(p.q_tiles, max(0, tile * kRows - off) / kRows);
+    tiles = p.q_tiles - first;
+  } else {
+    tile = p.q_tiles - 1 - (int)(x % p.q_tiles);
+    x /= p.q_tiles;
+    h = (int)(x % p.a.heads);
+    b = (int)(x / p.a.heads);
+    const int keys = p.a.causal ? max(0, min(p.a.kv_len, min((tile + 1) * kRows, p.a.q_len) + off)) : p.a.kv_len;
+    tiles = (keys + kRows - 1) / kRows;
+  }
+  const int row0 = tile * kRows;
+  const unsigned char* mask = MASK ? p.a.mask + b * p.a.mask_stride : nullptr;
+
+  if (threadIdx.x == 0) {
+    mbar_init(fixed, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    mbar_init(t1_full, 1);
+    mbar_init(t2_full, 1);
+    mbar_init(p_ready, 256);
+    mbar_init(ds_ready, 256);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (MASK && !KEYS)
+    pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS), mask, tiles, p.a.kv_len, warp, BWD_THREADS / 32, lane);
+  if (warp == ISSUER) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  bool dead_key = false;  // this thread's key row is masked
+  if (MASK && KEYS) {
+    const int j = row0 + (int)threadIdx.x % kRows;
+    dead_key = j < p.a.kv_len && !mask[j];
+  }
+  tc_fence_before();
+  // a tile of masked keys alone has nothing to do
+  if (MASK && KEYS) {
+    if (!__syncthreads_or(!dead_key && row0 + (int)threadIdx.x % kRows < p.a.kv_len)) tiles = 0;
+  } else {
+    __syncthreads();
+  }
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, t1 = tmem, t2 = tmem + 128, acc1 = tmem + 256, acc2 = tmem + 256 + 64 * PANELS;
+  const KeyBits bits{MASK && !KEYS ? reinterpret_cast<const uint4*>(smem + L::BITS) : nullptr};
+  // steps: query tiles of every head of the group, or tiles of keys of which some are seen
+  const int steps = KEYS ? tiles * p.a.group : tiles;
+  const int start = bits.next(0, steps);
+
+  if (warp == LOADER) {
+    if (lane == 0 && start < steps) {
+      mbar_arrive_expect_tx(fixed, 2 * L::TILE);
+#pragma unroll
+      for (int i = 0; i < PANELS; ++i) {
+        tma_load_4d(r1 + i * kPanel, KEYS ? &p.mk : &p.mq, fixed, i * 64, row0, h, b);
+        tma_load_4d(r2 + i * kPanel, KEYS ? &p.mv : &p.mdo, fixed, i * 64, row0, h, b);
+      }
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int j = start; ok && j < steps; j = bits.next(j + 1, steps)) {
+        const int t = KEYS ? first + j % tiles : j, hh = KEYS ? h * p.a.group + j / tiles : h / p.a.group;
+        for (int k = 0; k < 2; ++k) {
+          if (!(ok = mbar_wait(empty + s, ph ^ 1, abort_flag, status, ST_ATTN_LOAD))) break;
+          uint8_t* dst = ring + s * L::TILE;
+          const bool stats = KEYS && k == 0;
+          mbar_arrive_expect_tx(full + s, L::TILE + (stats ? 1024 : 0));
+          const CUtensorMap* map = KEYS ? (k ? &p.mdo : &p.mq) : (k ? &p.mv : &p.mk);
+#pragma unroll
+          for (int i = 0; i < PANELS; ++i) tma_load_4d(dst + i * kPanel, map, full + s, i * 64, t * kRows, hh, b);
+          if (stats)
+            bulk_load(smem + L::STATS + s / 2 * 1024, p.stats + (((long long)b * p.a.heads + hh) * p.q_tiles + t) * 256, 1024,
+                      full + s);
+          if (++s == STAGES) s = 0, ph ^= 1;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == ISSUER) {
+    if (lane == 0) {
+      const int ksteps = (p.a.head_dim + 15) / 16;
+      const uint32_t idesc_t = make_idesc(128, 128, umma_format<T>(), 0, 0);
+      const uint32_t idesc_a = make_idesc(128, ksteps * 16, umma_format<T>(), 0, 1);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        ok = ok && mbar_wait(bar, parity, abort_flag, status, ST_ATTN_MMA);
+        tc_fence_after();
+        return ok;
+      };
+      auto at = [&](int stage) { return smem_u32(ring + stage * L::TILE); };
+      int s = 0;
+      uint32_t ph = 0, pph = 0, more = 0;
+      int j = start;
+      if (j < steps && wait(fixed, 0) && wait(full, 0)) {
+        mma_scores(t1, smem_u32(r1), at(0), idesc_t, ksteps);
+        umma_commit(t1_full);
+        if (wait(full + 1, 0)) {
+          mma_scores(t2, smem_u32(r2), at(1), idesc_t, ksteps);
+          umma_commit(t2_full);
+          if (!KEYS) umma_commit(empty + 1);
+        }
+      }
+      while (ok && j < steps) {
+        const int cur = s;
+        s += 2;
+        if (s == STAGES) s = 0, ph ^= 1;
+        const int jn = bits.next(j + 1, steps);
+        if (!wait(p_ready, pph)) break;
+        if (KEYS) {
+          mma_probs(acc1, t1, at(cur + 1), idesc_a, more, 64);
+          umma_commit(empty + cur + 1);
+        }
+        if (jn < steps) {
+          if (!wait(full + s, ph)) break;
+          mma_scores(t1, smem_u32(r1), at(s), idesc_t, ksteps);
+          umma_commit(t1_full);
+        }
+        if (!wait(ds_ready, pph)) break;
+        mma_probs(acc2, t2, at(cur), idesc_a, more, 64);
+        umma_commit(empty + cur);
+        if (jn < steps) {
+          if (!wait(full + s + 1, ph)) break;
+          mma_scores(t2, smem_u32(r2), at(s + 1), idesc_t, ksteps);
+          umma_commit(t2_full);
+          if (!KEYS) umma_commit(empty + s + 1);
+        }
+        more = 1;
+        pph ^= 1;
+        j = jn;
+      }
+      // the sums are whole, and no product may be writing TMEM when it is released
+      umma_commit(done);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(done, 0))
+        if (globaltimer_ns() - t0 > LSR_WAIT_TIMEOUT_NS) {
+          set_status(status, ST_ATTN_DONE);
+          *abort_flag = 1;
+          break;
+        }
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    const int half = warp / 4, r = warp % 4 * 32 + lane, row = row0 + r;
+    const uint32_t quarter = (uint32_t)(warp % 4 * 32) << 16;
+    const uint32_t my1 = t1 + half * 64 + quarter, my2 = t2 + half * 64 + quarter;
+    const float c = p.a.scale * kLog2e;
+    bool ok = true;
+    uint32_t ph = 0;
+    int cur = 0;  // stage of the step's first tile
+    uint32_t sph = 0;
+    float lse = 0.f, delta = 0.f;
+    if (!KEYS) {
+      const float* st = p.stats + (((long long)b * p.a.heads + h) * p.q_tiles + tile) * 256 + r;
+      lse = st[0] + (float)kExtra<T>;
+      delta = st[128] * (float)(1 << kExtra<T>);
+    }
+    for (int j = start; j < steps; j = bits.next(j + 1, steps)) {
+      const int t0 = (KEYS ? first + j % tiles : j) * kRows + half * 64;  // position of the thread's first column
+      if (!(ok = warp_wait(t1_full, ph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
+      tc_fence_after();
+      uint32_t s[2][32];
+      tmem_ld32(my1, s[0]);
+      tmem_ld32(my1 + 32, s[1]);
+      // the statistics came with the step's first tile, which the product above has waited for
+      const float4* stat = reinterpret_cast<const float4*>(smem + L::STATS + cur / 2 * 1024) + half * 16;
+      if (KEYS && !(ok = warp_wait(full + cur, sph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
+      tmem_ld_wait();
+      uint2 word = make_uint2(~0u, ~0u);  // which of the thread's keys are seen
+      if (MASK && !KEYS) {
+        const uint4 w = bits.bits[j];
+        word = half ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y);
+      }
+      const bool holes = MASK && !KEYS && (word.x & word.y) != ~0u;
+      if (KEYS) {
+        if (p.a.causal && row0 + kRows - 1 > t0 + off) {
+          const int from = row - off - t0;  // queries before it do not see the key
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (e < from) s[e / 32][e % 32] = 0xff800000u;
+        }
+      } else {
+        const int sees = min(p.a.kv_len, p.a.causal ? row + off + 1 : p.a.kv_len) - t0;
+        if (holes || t0 + 64 > p.a.kv_len || (p.a.causal && t0 + 63 > row0 + off)) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (e >= sees || (MASK && !(((e < 32 ? word.x : word.y) >> (e % 32)) & 1))) s[e / 32][e % 32] = 0xff800000u;
+        }
+        tc_fence_before();
+        mbar_arrive(p_ready);  // T1 is in registers
+      }
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        const float4 v = KEYS ? stat[e / 4] : make_float4(lse, lse, lse, lse);
+        uint32_t* q = &s[e / 32][e % 32];
+        q[0] = __float_as_uint(ex2(fmaf(__uint_as_float(q[0]), c, -v.x)));
+        q[1] = __float_as_uint(ex2(fmaf(__uint_as_float(q[1]), c, -v.y)));
+        q[2] = __float_as_uint(ex2(fmaf(__uint_as_float(q[2]), c, -v.z)));
+        q[3] = __float_as_uint(ex2(fmaf(__uint_as_float(q[3]), c, -v.w)));
+      }
+      if (KEYS) {
+        uint32_t pr[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          pr[e] = pack2<T>(__uint_as_float(s[e / 16][e % 16 * 2]), __uint_as_float(s[e / 16][e % 16 * 2 + 1]));
+        tmem_st32(my1, pr);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(p_ready);
+      }
+      if (!(ok = warp_wait(t2_full, ph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
+      tc_fence_after();
+      uint32_t d[2][32], pr[32];
+      tmem_ld32(my2, d[0]);
+      tmem_ld32(my2 + 32, d[1]);
+      tmem_ld_wait();
+      if (holes) {  // what a hidden key's values hold must not reach 0 times it
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (!(((e < 32 ? word.x : word.y) >> (e % 32)) & 1)) d[e / 32][e % 32] = 0;
+      }
+      constexpr float kDown = 1.f / (1 << (KEYS ? kExtra<T> : 0));
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        const float4 v = KEYS ? stat[32 + e / 4] : make_float4(delta, delta, delta, delta);
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float dp = __uint_as_float(d[(e + k) / 32][(e + k) % 32]);
+          const float dl = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
+          x[k] = __uint_as_float(s[(e + k) / 32][(e + k) % 32]) * (kDown == 1.f ? dp - dl : fmaf(dp, kDown, -dl));
+        }
+        pr[e / 2] = pack2<T>(x[0], x[1]);
+        pr[e / 2 + 1] = pack2<T>(x[2], x[3]);
+      }
+      tmem_st32(my2, pr);
+      if (MASK && !KEYS) {  // nor what its keys hold
+        const uint4 w = bits.bits[j];
+        const uint32_t wr = r < 32 ? w.x : r < 64 ? w.y : r < 96 ? w.z : w.w;
+        if (!((wr >> lane) & 1) && half < PANELS) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(ring + cur * L::TILE + half * kPanel + r * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(ds_ready);
+      ph ^= 1;
+      cur += 2;
+      if (cur == STAGES) cur = 0, sph ^= 1;
+    }
+    if (ok) ok = warp_wait(done, 0, abort_flag, status, ST_ATTN_SOFTMAX);
+    tc_fence_after();
+    if (ok) {
+      const bool any = start < steps && !dead_key;
+      if (KEYS) {
+        const bool live = row < p.a.kv_len;
+        if (half == 0)
+          store_rows(attn_at<T>(p.a.dv, p.a.sdv, b, h) + row * p.a.sdv.s, acc1 + quarter, 0, 64 * PANELS, p.a.head_dim, live, any,
+                     1.f / (1 << kExtra<T>));
+        else
+          store_rows(attn_at<T>(p.a.dk, p.a.sdk, b, h) + row * p.a.sdk.s, acc2 + quarter, 0, 64 * PANELS, p.a.head_dim, live, any,
+                     p.a.scale);
+      } else {
+        store_rows(attn_at<T>(p.a.dq, p.a.sdq, b, h) + row * p.a.sdq.s, acc2 + quarter, half * 32 * PANELS,
+                   (half + 1) * 32 * PANELS, p.a.head_dim, row < p.a.q_len, any, p.a.scale);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == ISSUER) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int PANELS, bool MASK>
+__global__ void __launch_bounds__(BWD_THREADS, 1) attn_bwd_kernel(const __grid_constant__ BwdParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;
+  if (blockIdx.x < p.kv_blocks) bwd_block<T, PANELS, MASK, true>(p, blockIdx.x, smem);
+  else bwd_block<T, PANELS, MASK, false>(p, blockIdx.x - (unsigned)p.kv_blocks, smem);
+}
+
+template <typename T, int PANELS, bool MASK>
+int launch(BwdParams& p, cudaStream_t st) {
+  using L = BwdSmem<PANELS, MASK>;
+  static_assert(L::TOTAL <= 232448, "shared memory budget exceeded");
+  const long long rows = (long long)p.q_tiles * kRows * p.a.heads * p.a.batch;
+  const long long blocks = p.kv_blocks + (long long)p.q_tiles * p.a.heads * p.a.batch;
+  if (blocks > 0x7fffffffll || rows / 32 > 0x7fffffffll) return LSR_ERR_SHAPE;
+  {
+    ProfScope prof(PK_EW_OTHER, st);
+    attn_stats_kernel<T><<<(unsigned)(rows / 32), 256, 0, st>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return LSR_ERR_LAUNCH;
+  }
+  auto kernel = attn_bwd_kernel<T, PANELS, MASK>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess)
+    return LSR_ERR_LAUNCH;
+  ProfScope prof(PK_GEMM_OTHER, st);
+  kernel<<<(unsigned)blocks, BWD_THREADS, L::TOTAL, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
+}
+
+template <typename T>
+int backward(BwdParams& p, cudaStream_t st) {
+  if (p.a.head_dim > 64) return p.a.mask ? launch<T, 2, true>(p, st) : launch<T, 2, false>(p, st);
+  return p.a.mask ? launch<T, 1, true>(p, st) : launch<T, 1, false>(p, st);
+}
+
+}  // namespace
+
+size_t attention_backward_sm100_ws(const AttnParams& p) {
+  return (size_t)cdiv(p.q_len, kRows) * p.heads * p.batch * 256 * sizeof(float);
+}
+
+int attention_backward_sm100(const AttnParams& a, int dtype, void* ws, cudaStream_t st) {
+  BwdParams p{};
+  p.a = a;
+  p.stats = static_cast<float*>(ws);
+  p.q_tiles = cdiv(a.q_len, kRows);
+  p.kv_tiles = cdiv(a.kv_len, kRows);
+  p.kv_blocks = (long long)p.kv_tiles * a.kv_heads * a.batch;
+  int rc = encode_rows(&p.mq, a.q, a.sq, a.batch, a.heads, a.q_len, a.head_dim, dtype);
+  if (rc == LSR_OK) rc = encode_rows(&p.mdo, a.dout, a.sdo, a.batch, a.heads, a.q_len, a.head_dim, dtype);
+  if (rc == LSR_OK) rc = encode_rows(&p.mk, a.k, a.sk, a.batch, a.kv_heads, a.kv_len, a.head_dim, dtype);
+  if (rc == LSR_OK) rc = encode_rows(&p.mv, a.v, a.sv, a.batch, a.kv_heads, a.kv_len, a.head_dim, dtype);
+  if (rc != LSR_OK) return rc;
+  return dtype == LSR_DTYPE_BF16 ? backward<__nv_bfloat16>(p, st) : backward<__half>(p, st);
+}
+
+}  // namespace lsr

@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1) attn_fwd_kerne
         for (int w = 0; ok && w < NQ; ++w) {
           if (j < n[w]) {
             if (!wait(p_ready + w, pph)) break;
-            mma_probs(o_at(w), s_at(w), smem_u32(skv + vs * L::TILE), idesc_o, (started >> w) & 1);
+            mma_probs(o_at(w), s_at(w), smem_u32(skv + vs * L::TILE), idesc_o, (started >> w) & 1, 32);
             started |= 1u << w;
             if (jn >= n[w]) umma_commit(o_full + w);
           }

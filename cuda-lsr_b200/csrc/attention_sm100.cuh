@@ -89,15 +89,14 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_smem, uint32_t
   }
 }
 
-// D (128 x entries) (+)= P B over 16-row steps [k0, k1) of the tile B: P in TMEM.
+// D (128 x entries) (+)= P B over the tile B's 128 rows: P in TMEM, the operand of the second 64 rows
+// `half` columns after that of the first.
 __device__ __forceinline__ void mma_probs(uint32_t d, uint32_t p_tmem, uint32_t b_smem, uint32_t idesc, uint32_t accumulate,
-                                          int k0 = 0, int k1 = 8) {
+                                          int half) {
   const uint64_t b = smem_desc_sw128(b_smem, kPanel, 1024);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if (k < k0 || k >= k1) continue;
-    umma_ts(d, p_tmem + k * 8, b + (uint64_t)(k * (2048 >> 4)), idesc, accumulate || k > k0);
-  }
+  for (int k = 0; k < 8; ++k)
+    umma_ts(d, p_tmem + (k >> 2) * half + (k & 3) * 8, b + (uint64_t)(k * (2048 >> 4)), idesc, accumulate || k > 0);
 }
 
 // One tile of [position][entry], panel by panel.
@@ -141,5 +140,7 @@ bool rows_ok(const void* base, const AttnStride& s, int batch, int heads, int le
 
 int attention_forward_sm100(const AttnParams& p, int dtype, void* ws, cudaStream_t st);
 size_t attention_forward_sm100_ws(const AttnParams& p);
+int attention_backward_sm100(const AttnParams& p, int dtype, void* ws, cudaStream_t st);
+size_t attention_backward_sm100_ws(const AttnParams& p);
 
 }  // namespace lsr

@@ -125,7 +125,7 @@ def attention_backward(dout, q, k, v, out, lse, *, causal: bool = False, scale: 
         args = _pack(q, k, v, key_mask, causal, _scale(scale, q), out, lse, dout, dq, dk, dv)
         nbytes = lib.lsr_attention_backward_workspace_bytes(args)
         ws = _workspace(nbytes, q.device)
-        rc = lib.lsr_attention_backward(args, ws.data_ptr(), nbytes, _lib.stream_handle(q.device))
+        rc = lib.lsr_attention_backward(args, ws.data_ptr() if nbytes else None, nbytes, _lib.stream_handle(q.device))
     _lib.check(rc, "lsr_attention_backward")
     return dq, dk, dv
 
