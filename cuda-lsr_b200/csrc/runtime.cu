@@ -141,6 +141,17 @@ int check_device() {
 }
 
 namespace {
+// The driver's encoder wants a context on the calling thread, and a thread that has made no other runtime
+// call (an autograd worker in its first backward pass) has none yet: cudaSetDevice binds it.
+template <typename... A>
+CUresult encode_bound(EncodeTiledFn encode, A... args) {
+  const CUresult r = encode(args...);
+  if (r == CUDA_SUCCESS) return r;
+  const int d = current_device();
+  if (d < 0 || cudaSetDevice(d) != cudaSuccess) return r;
+  return encode(args...);
+}
+
 EncodeTiledFn encode_fn() {
   EncodeTiledFn encode = g_encode.load(std::memory_order_relaxed);
   if (!encode) {
@@ -170,7 +181,7 @@ int encode_tmap_k_blocks(CUtensorMap* map, CUtensorMapDataType dtype, int elem_b
   cuuint64_t strides[3] = {ld * elem_bytes, block * elem_bytes, bstride * elem_bytes};
   cuuint32_t box[4] = {(cuuint32_t)block, box_rows, box_blocks, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = encode(map, dtype, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode_bound(encode, map, dtype, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? LSR_OK : LSR_ERR_DRIVER;
 }
@@ -188,7 +199,7 @@ int encode_tmap_mn_chunks(CUtensorMap* map, CUtensorMapDataType dtype, int elem_
   cuuint64_t strides[3] = {ld * elem_bytes, chunk * elem_bytes, bstride * elem_bytes};
   cuuint32_t box[4] = {(cuuint32_t)chunk, box_krows, box_chunks, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = encode(map, dtype, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode_bound(encode, map, dtype, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? LSR_OK : LSR_ERR_DRIVER;
 }
@@ -200,7 +211,7 @@ int encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
   if ((reinterpret_cast<uintptr_t>(base) & 15) || ((strides[0] | strides[1] | strides[2]) & 15)) return LSR_ERR_SHAPE;
   cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, st[3] = {strides[0], strides[1], strides[2]};
   cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]}, estr[4] = {1, 1, 1, 1};
-  CUresult r = encode(map, dtype, 4, const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode_bound(encode, map, dtype, 4, const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? LSR_OK : LSR_ERR_DRIVER;
 }
@@ -208,17 +219,8 @@ int encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base
 int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, int elem_bytes, const void* base, uint64_t inner,
                    uint64_t outer, uint64_t batch, uint64_t ld, uint64_t bstride, uint32_t box_inner,
                    uint32_t box_outer, CUtensorMapSwizzle swizzle) {
-  EncodeTiledFn encode = g_encode.load(std::memory_order_relaxed);
-  if (!encode) {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) !=
-            cudaSuccess ||
-        q != cudaDriverEntryPointSuccess || !fn)
-      return LSR_ERR_DRIVER;
-    encode = reinterpret_cast<EncodeTiledFn>(fn);
-    g_encode.store(encode, std::memory_order_relaxed);
-  }
+  EncodeTiledFn encode = encode_fn();
+  if (!encode) return LSR_ERR_DRIVER;
   // TMA requirements: 16-byte aligned base and strides.
   if ((reinterpret_cast<uintptr_t>(base) & 15) || ((ld * elem_bytes) & 15) || ((bstride * elem_bytes) & 15))
     return LSR_ERR_SHAPE;
@@ -226,7 +228,7 @@ int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, int elem_bytes, 
   cuuint64_t strides[2] = {ld * elem_bytes, bstride * elem_bytes};
   cuuint32_t box[3] = {box_inner, box_outer, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = encode(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode_bound(encode, map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? LSR_OK : LSR_ERR_DRIVER;

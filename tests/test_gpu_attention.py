@@ -312,6 +312,33 @@ def test_captured_and_replayed():
         assert all(torch.equal(x, y) for x, y in zip(r, want))
 
 
+def test_a_thread_whose_first_call_this_is():
+    """As an autograd worker's first backward pass: the thread has no CUDA context of its own yet."""
+    import threading
+    from lsr import attention as A
+    q, k, v, do = tensors(1, 70, 70, 2, 2, 64, torch.bfloat16, seed=12)
+    o, lse = A.attention_forward(q, k, v, causal=True)
+    want = (o, lse) + tuple(A.attention_backward(do, q, k, v, o, lse, causal=True))
+    torch.cuda.synchronize()
+    got = []
+
+    def work(backward_first):
+        try:
+            grads = A.attention_backward(do, q, k, v, o, lse, causal=True) if backward_first else ()
+            got.append(tuple(A.attention_forward(q, k, v, causal=True)) + tuple(grads))
+        except Exception as e:  # noqa: BLE001
+            got.append(e)
+
+    for first in (True, False):
+        t = threading.Thread(target=work, args=(first,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    for r in got:
+        assert not isinstance(r, Exception), r
+        assert all(torch.equal(x, y) for x, y in zip(r, want))
+
+
 def test_nothing_to_do():
     from lsr import attention as A
     for b, n, m in ((0, 5, 5), (2, 0, 5), (2, 5, 0)):
