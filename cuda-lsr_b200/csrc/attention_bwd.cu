@@ -14,6 +14,8 @@
 // overwrites T1 and dS overwrites T2 as 16-bit operands. The products of one step and the scores of the
 // next are issued as their operands get ready: while the threads take the exponentials of T1, the
 // tensor core adds dS and computes the next T2; while they form dS, it adds P and computes the next T1.
+// Sixteen warps share a tile's scores, 32 columns a thread: with eight the waits on TMEM and on the special
+// function units showed more (4 x 16 heads x 4096 x 64: 1267 us, now 1170, 587 TFLOP/s; dim 128: 1853 us, 742).
 // P and dS are rounded to 16 bits for the products. In fp16 P is taken times 2^10 (at most 1024), so
 // that rows over thousands of keys stay above its smallest normal value; dV is scaled back.
 #include "attention_sm100.cuh"
@@ -21,8 +23,12 @@
 namespace lsr {
 namespace {
 
-constexpr int BWD_THREADS = 384;  // two warpgroups on the scores, then the loader, the issuer and two idle warps
-constexpr int LOADER = 8, ISSUER = 9;
+constexpr int PARTS = 4;  // warpgroups on the scores, each with 128 / PARTS columns
+constexpr int COLS = kRows / PARTS;
+constexpr int BWD_THREADS = PARTS * 128 + 128;  // then the loader, the issuer and two idle warps
+constexpr int LOADER = 4 * PARTS, ISSUER = LOADER + 1;
+// Registers a thread after the split, within the 96 that five warpgroups are launched with: 5 x 96 = 4 x 104 + 64.
+constexpr int kScoreRegs = 104, kRestRegs = 64;
 
 // Extra power of two in P.
 template <typename T>
@@ -116,7 +122,8 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
            *p_ready = t2_full + 1, *ds_ready = p_ready + 1, *done = ds_ready + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // the same in all lanes, and known to be: the roles below then run as uniform code
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int off = p.a.kv_len - p.a.q_len;  // under causality query i sees keys up to i + off
   int* status = p.a.status;
 
@@ -148,8 +155,8 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
     }
     mbar_init(t1_full, 1);
     mbar_init(t2_full, 1);
-    mbar_init(p_ready, 256);
-    mbar_init(ds_ready, 256);
+    mbar_init(p_ready, 4 * PARTS);
+    mbar_init(ds_ready, 4 * PARTS);
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -179,89 +186,100 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
   const int steps = KEYS ? tiles * p.a.group : tiles;
   const int start = bits.next(0, steps);
 
-  if (warp == LOADER) {
-    if (lane == 0 && start < steps) {
-      mbar_arrive_expect_tx(fixed, 2 * L::TILE);
+  if (warp >= LOADER) {
+    regs_dec<kRestRegs>();
+    if (warp == LOADER) {
+      if (lane == 0 && start < steps) {
+        mbar_arrive_expect_tx(fixed, 2 * L::TILE);
 #pragma unroll
-      for (int i = 0; i < PANELS; ++i) {
-        tma_load_4d(r1 + i * kPanel, KEYS ? &p.mk : &p.mq, fixed, i * 64, row0, h, b);
-        tma_load_4d(r2 + i * kPanel, KEYS ? &p.mv : &p.mdo, fixed, i * 64, row0, h, b);
-      }
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int j = start; ok && j < steps; j = bits.next(j + 1, steps)) {
-        const int t = KEYS ? first + j % tiles : j, hh = KEYS ? h * p.a.group + j / tiles : h / p.a.group;
-        for (int k = 0; k < 2; ++k) {
-          if (!(ok = mbar_wait(empty + s, ph ^ 1, abort_flag, status, ST_ATTN_LOAD))) break;
-          uint8_t* dst = ring + s * L::TILE;
-          const bool stats = KEYS && k == 0;
-          mbar_arrive_expect_tx(full + s, L::TILE + (stats ? 1024 : 0));
-          const CUtensorMap* map = KEYS ? (k ? &p.mdo : &p.mq) : (k ? &p.mv : &p.mk);
+        for (int i = 0; i < PANELS; ++i) {
+          tma_load_4d(r1 + i * kPanel, KEYS ? &p.mk : &p.mq, fixed, i * 64, row0, h, b);
+          tma_load_4d(r2 + i * kPanel, KEYS ? &p.mv : &p.mdo, fixed, i * 64, row0, h, b);
+        }
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int j = start; ok && j < steps; j = bits.next(j + 1, steps)) {
+          const int t = KEYS ? first + j % tiles : j, hh = KEYS ? h * p.a.group + j / tiles : h / p.a.group;
+          for (int k = 0; k < 2; ++k) {
+            if (!(ok = mbar_wait(empty + s, ph ^ 1, abort_flag, status, ST_ATTN_LOAD))) break;
+            uint8_t* dst = ring + s * L::TILE;
+            const bool stats = KEYS && k == 0;
+            mbar_arrive_expect_tx(full + s, L::TILE + (stats ? 1024 : 0));
+            const CUtensorMap* map = KEYS ? (k ? &p.mdo : &p.mq) : (k ? &p.mv : &p.mk);
 #pragma unroll
-          for (int i = 0; i < PANELS; ++i) tma_load_4d(dst + i * kPanel, map, full + s, i * 64, t * kRows, hh, b);
-          if (stats)
-            bulk_load(smem + L::STATS + s / 2 * 1024, p.stats + (((long long)b * p.a.heads + hh) * p.q_tiles + t) * 256, 1024,
-                      full + s);
-          if (++s == STAGES) s = 0, ph ^= 1;
+            for (int i = 0; i < PANELS; ++i) tma_load_4d(dst + i * kPanel, map, full + s, i * 64, t * kRows, hh, b);
+            if (stats)
+              bulk_load(smem + L::STATS + s / 2 * 1024, p.stats + (((long long)b * p.a.heads + hh) * p.q_tiles + t) * 256, 1024,
+                        full + s);
+            if (++s == STAGES) s = 0, ph ^= 1;
+          }
         }
       }
-    }
-    __syncwarp();
-  } else if (warp == ISSUER) {
-    if (lane == 0) {
+      __syncwarp();
+    } else if (warp == ISSUER) {
+      // The whole warp runs along, so that addresses and descriptors stay in uniform registers; one lane issues.
       const int ksteps = (p.a.head_dim + 15) / 16;
       const uint32_t idesc_t = make_idesc(128, 128, umma_format<T>(), 0, 0);
       const uint32_t idesc_a = make_idesc(128, ksteps * 16, umma_format<T>(), 0, 1);
+      const uint32_t ra1 = smem_u32(r1), ra2 = smem_u32(r2), xa = smem_u32(ring);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && mbar_wait(bar, parity, abort_flag, status, ST_ATTN_MMA);
+        ok = ok && warp_wait(bar, parity, abort_flag, status, ST_ATTN_MMA);
         tc_fence_after();
         return ok;
       };
-      auto at = [&](int stage) { return smem_u32(ring + stage * L::TILE); };
-      int s = 0;
+      int s = 0;  // stage of the step's first tile; the second lies in the next (the stage count is even)
       uint32_t ph = 0, pph = 0, more = 0;
+      auto scores1 = [&] {
+        mma_scores<PANELS>(t1, ra1, xa + s * L::TILE, idesc_t, ksteps);
+        umma_commit(t1_full);
+      };
+      auto scores2 = [&] {
+        mma_scores<PANELS>(t2, ra2, xa + (s + 1) * L::TILE, idesc_t, ksteps);
+        umma_commit(t2_full);
+        if (!KEYS) umma_commit(empty + s + 1);
+      };
       int j = start;
       if (j < steps && wait(fixed, 0) && wait(full, 0)) {
-        mma_scores(t1, smem_u32(r1), at(0), idesc_t, ksteps);
-        umma_commit(t1_full);
+        if (elect_one()) scores1();
+        __syncwarp();
         if (wait(full + 1, 0)) {
-          mma_scores(t2, smem_u32(r2), at(1), idesc_t, ksteps);
-          umma_commit(t2_full);
-          if (!KEYS) umma_commit(empty + 1);
+          if (elect_one()) scores2();
+          __syncwarp();
         }
       }
       while (ok && j < steps) {
-        const int cur = s;
+        const uint32_t x1 = xa + s * L::TILE, x2 = x1 + L::TILE;
+        uint64_t* left = empty + s;
         s += 2;
         if (s == STAGES) s = 0, ph ^= 1;
         const int jn = bits.next(j + 1, steps);
+        if (jn < steps && !wait(full + s, ph)) break;
         if (!wait(p_ready, pph)) break;
-        if (KEYS) {
-          mma_probs(acc1, t1, at(cur + 1), idesc_a, more, 64);
-          umma_commit(empty + cur + 1);
+        if (elect_one()) {
+          if (KEYS) {
+            mma_probs<128, COLS, COLS>(acc1, t1, x2, idesc_a, more);
+            umma_commit(left + 1);
+          }
+          if (jn < steps) scores1();
         }
-        if (jn < steps) {
-          if (!wait(full + s, ph)) break;
-          mma_scores(t1, smem_u32(r1), at(s), idesc_t, ksteps);
-          umma_commit(t1_full);
-        }
+        __syncwarp();
+        if (jn < steps && !wait(full + s + 1, ph)) break;
         if (!wait(ds_ready, pph)) break;
-        mma_probs(acc2, t2, at(cur), idesc_a, more, 64);
-        umma_commit(empty + cur);
-        if (jn < steps) {
-          if (!wait(full + s + 1, ph)) break;
-          mma_scores(t2, smem_u32(r2), at(s + 1), idesc_t, ksteps);
-          umma_commit(t2_full);
-          if (!KEYS) umma_commit(empty + s + 1);
+        if (elect_one()) {
+          mma_probs<128, COLS, COLS>(acc2, t2, x1, idesc_a, more);
+          umma_commit(left);
+          if (jn < steps) scores2();
         }
+        __syncwarp();
         more = 1;
         pph ^= 1;
         j = jn;
       }
       // the sums are whole, and no product may be writing TMEM when it is released
-      umma_commit(done);
+      if (elect_one()) umma_commit(done);
+      __syncwarp();
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(done, 0))
         if (globaltimer_ns() - t0 > LSR_WAIT_TIMEOUT_NS) {
@@ -269,13 +287,15 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
           *abort_flag = 1;
           break;
         }
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp < 8) {
-    const int half = warp / 4, r = warp % 4 * 32 + lane, row = row0 + r;
+  } else {
+    regs_inc<kScoreRegs>();
+    const int part = warp / 4, r = warp % 4 * 32 + lane, row = row0 + r;
     const uint32_t quarter = (uint32_t)(warp % 4 * 32) << 16;
-    const uint32_t my1 = t1 + half * 64 + quarter, my2 = t2 + half * 64 + quarter;
+    const uint32_t my1 = t1 + part * COLS + quarter, my2 = t2 + part * COLS + quarter;
     const float c = p.a.scale * kLog2e;
+    const uint64_t c2 = pair(c, c);
     bool ok = true;
     uint32_t ph = 0;
     int cur = 0;  // stage of the step's first tile
@@ -287,97 +307,87 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
       delta = st[128] * (float)(1 << kExtra<T>);
     }
     for (int j = start; j < steps; j = bits.next(j + 1, steps)) {
-      const int t0 = (KEYS ? first + j % tiles : j) * kRows + half * 64;  // position of the thread's first column
+      const int t0 = (KEYS ? first + j % tiles : j) * kRows + part * COLS;  // position of the thread's first column
+      // the statistics come with the step's first tile
+      if (KEYS && !(ok = warp_wait(full + cur, sph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
+      const float4* stat = reinterpret_cast<const float4*>(smem + L::STATS + cur / 2 * 1024) + part * (COLS / 4);
       if (!(ok = warp_wait(t1_full, ph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
       tc_fence_after();
-      uint32_t s[2][32];
-      tmem_ld32(my1, s[0]);
-      tmem_ld32(my1 + 32, s[1]);
-      // the statistics came with the step's first tile, which the product above has waited for
-      const float4* stat = reinterpret_cast<const float4*>(smem + L::STATS + cur / 2 * 1024) + half * 16;
-      if (KEYS && !(ok = warp_wait(full + cur, sph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
+      uint32_t s[COLS];
+      tmem_ld32(my1, s);
       tmem_ld_wait();
-      uint2 word = make_uint2(~0u, ~0u);  // which of the thread's keys are seen
-      if (MASK && !KEYS) {
-        const uint4 w = bits.bits[j];
-        word = half ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y);
-      }
-      const bool holes = MASK && !KEYS && (word.x & word.y) != ~0u;
+      uint32_t word = ~0u;  // which of the thread's keys are seen
+      if (MASK && !KEYS) word = reinterpret_cast<const uint32_t*>(bits.bits + j)[part];
       if (KEYS) {
         if (p.a.causal && row0 + kRows - 1 > t0 + off) {
           const int from = row - off - t0;  // queries before it do not see the key
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (e < from) s[e / 32][e % 32] = 0xff800000u;
+          for (int e = 0; e < COLS; ++e)
+            if (e < from) s[e] = 0xff800000u;
         }
       } else {
+        warp_arrive(p_ready, lane);  // T1 is in registers
         const int sees = min(p.a.kv_len, p.a.causal ? row + off + 1 : p.a.kv_len) - t0;
-        if (holes || t0 + 64 > p.a.kv_len || (p.a.causal && t0 + 63 > row0 + off)) {
+        if (word != ~0u || t0 + COLS > p.a.kv_len || (p.a.causal && t0 + COLS - 1 > row0 + off)) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (e >= sees || (MASK && !(((e < 32 ? word.x : word.y) >> (e % 32)) & 1))) s[e / 32][e % 32] = 0xff800000u;
+          for (int e = 0; e < COLS; ++e)
+            if (e >= sees || (MASK && !((word >> e) & 1))) s[e] = 0xff800000u;
         }
-        tc_fence_before();
-        mbar_arrive(p_ready);  // T1 is in registers
       }
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
+      for (int e = 0; e < COLS; e += 4) {
         const float4 v = KEYS ? stat[e / 4] : make_float4(lse, lse, lse, lse);
-        uint32_t* q = &s[e / 32][e % 32];
-        q[0] = __float_as_uint(ex2(fmaf(__uint_as_float(q[0]), c, -v.x)));
-        q[1] = __float_as_uint(ex2(fmaf(__uint_as_float(q[1]), c, -v.y)));
-        q[2] = __float_as_uint(ex2(fmaf(__uint_as_float(q[2]), c, -v.z)));
-        q[3] = __float_as_uint(ex2(fmaf(__uint_as_float(q[3]), c, -v.w)));
+        float x[4];
+        unpair(fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, pair(-v.x, -v.y)), x[0], x[1]);
+        unpair(fma2(pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), c2, pair(-v.z, -v.w)), x[2], x[3]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[e + k] = __float_as_uint(ex2(x[k]));
       }
       if (KEYS) {
-        uint32_t pr[32];
+        uint32_t pr[COLS / 2];
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          pr[e] = pack2<T>(__uint_as_float(s[e / 16][e % 16 * 2]), __uint_as_float(s[e / 16][e % 16 * 2 + 1]));
-        tmem_st32(my1, pr);
+        for (int e = 0; e < COLS / 2; ++e) pr[e] = pack2<T>(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+        tmem_st16(my1, pr);
         tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(p_ready);
+        warp_arrive(p_ready, lane);
       }
       if (!(ok = warp_wait(t2_full, ph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
       tc_fence_after();
-      uint32_t d[2][32], pr[32];
-      tmem_ld32(my2, d[0]);
-      tmem_ld32(my2 + 32, d[1]);
+      uint32_t d[COLS], pr[COLS / 2];
+      tmem_ld32(my2, d);
       tmem_ld_wait();
-      if (holes) {  // what a hidden key's values hold must not reach 0 times it
+      if (word != ~0u) {  // what a hidden key's values hold must not reach 0 times it
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (!(((e < 32 ? word.x : word.y) >> (e % 32)) & 1)) d[e / 32][e % 32] = 0;
+        for (int e = 0; e < COLS; ++e)
+          if (!((word >> e) & 1)) d[e] = 0;
       }
       constexpr float kDown = 1.f / (1 << (KEYS ? kExtra<T> : 0));
+      const uint64_t down = pair(kDown, kDown);
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
+      for (int e = 0; e < COLS; e += 4) {
         const float4 v = KEYS ? stat[32 + e / 4] : make_float4(delta, delta, delta, delta);
+        const uint64_t a0 = pair(__uint_as_float(d[e]), __uint_as_float(d[e + 1]));
+        const uint64_t a1 = pair(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3]));
+        const uint64_t m0 = pair(-v.x, -v.y), m1 = pair(-v.z, -v.w);
         float x[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float dp = __uint_as_float(d[(e + k) / 32][(e + k) % 32]);
-          const float dl = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
-          x[k] = __uint_as_float(s[(e + k) / 32][(e + k) % 32]) * (kDown == 1.f ? dp - dl : fmaf(dp, kDown, -dl));
-        }
+        unpair(mul2(kDown == 1.f ? add2(a0, m0) : fma2(a0, down, m0), pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1]))), x[0], x[1]);
+        unpair(mul2(kDown == 1.f ? add2(a1, m1) : fma2(a1, down, m1), pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]))), x[2],
+               x[3]);
         pr[e / 2] = pack2<T>(x[0], x[1]);
         pr[e / 2 + 1] = pack2<T>(x[2], x[3]);
       }
-      tmem_st32(my2, pr);
+      tmem_st16(my2, pr);
       if (MASK && !KEYS) {  // nor what its keys hold
-        const uint4 w = bits.bits[j];
-        const uint32_t wr = r < 32 ? w.x : r < 64 ? w.y : r < 96 ? w.z : w.w;
-        if (!((wr >> lane) & 1) && half < PANELS) {
+        const uint32_t seen = reinterpret_cast<const uint32_t*>(bits.bits + j)[r / 32];
+        if (!((seen >> lane) & 1) && part < PANELS) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<uint4*>(ring + cur * L::TILE + half * kPanel + r * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(ring + cur * L::TILE + part * kPanel + r * 128 + e * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
       tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(ds_ready);
+      warp_arrive(ds_ready, lane);
       ph ^= 1;
       cur += 2;
       if (cur == STAGES) cur = 0, sph ^= 1;
@@ -386,17 +396,19 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
     tc_fence_after();
     if (ok) {
       const bool any = start < steps && !dead_key;
-      if (KEYS) {
-        const bool live = row < p.a.kv_len;
-        if (half == 0)
-          store_rows(attn_at<T>(p.a.dv, p.a.sdv, b, h) + row * p.a.sdv.s, acc1 + quarter, 0, 64 * PANELS, p.a.head_dim, live, any,
+      if (KEYS) {  // half of the warpgroups store dv, half dk, each its share of the columns
+        constexpr int SHARE = 64 * PANELS / (PARTS / 2);
+        const bool live = row < p.a.kv_len, second = part >= PARTS / 2;
+        const int col = part % (PARTS / 2) * SHARE;
+        if (!second)
+          store_rows(attn_at<T>(p.a.dv, p.a.sdv, b, h) + row * p.a.sdv.s, acc1 + quarter, col, col + SHARE, p.a.head_dim, live, any,
                      1.f / (1 << kExtra<T>));
         else
-          store_rows(attn_at<T>(p.a.dk, p.a.sdk, b, h) + row * p.a.sdk.s, acc2 + quarter, 0, 64 * PANELS, p.a.head_dim, live, any,
+          store_rows(attn_at<T>(p.a.dk, p.a.sdk, b, h) + row * p.a.sdk.s, acc2 + quarter, col, col + SHARE, p.a.head_dim, live, any,
                      p.a.scale);
-      } else {
-        store_rows(attn_at<T>(p.a.dq, p.a.sdq, b, h) + row * p.a.sdq.s, acc2 + quarter, half * 32 * PANELS,
-                   (half + 1) * 32 * PANELS, p.a.head_dim, row < p.a.q_len, any, p.a.scale);
+      } else if (part < 2 * PANELS) {
+        store_rows(attn_at<T>(p.a.dq, p.a.sdq, b, h) + row * p.a.sdq.s, acc2 + quarter, part * 32, part * 32 + 32, p.a.head_dim,
+                   row < p.a.q_len, any, p.a.scale);
       }
     }
   }

@@ -5,11 +5,15 @@
 //   at the end:    out = O / l,  lse = (m c + log2 l) ln 2
 //
 // A block owns NQ tiles of 128 queries of one head and passes once over its keys. Warp 4 NQ loads
-// (TMA, a ring of key and value tiles), one thread of warp 4 NQ + 1 issues the products, and one
-// warpgroup per query tile does the softmax, a thread per query: a row's maximum and sum need no
-// exchange. S and O stay in TMEM; P goes back to TMEM over S as the 16-bit operand of P V, so scores
-// and probabilities never touch shared memory. While one query tile is in its softmax the tensor core
-// works for the other.
+// (TMA, a ring of key and value tiles), the warps after it issue the products, and one warpgroup per
+// query tile does the softmax, a thread per query: a row's maximum and sum need no exchange. S and O
+// stay in TMEM; P goes back to TMEM as the 16-bit operand of P V, so scores and probabilities never
+// touch shared memory. While one query tile is in its softmax the tensor core works for the other.
+// What bounds it: per 128 x 128 tile the exponentials take 1024 cycles of the special function units and
+// the products 1024 cycles of the tensor core at dim 128, 512 at dim 64. Measured (bf16, 4 x 16 heads x
+// 4096, no mask): dim 128 467 us, 1177 TFLOP/s; dim 64 360 us, 763 TFLOP/s, where those units are busy two
+// thirds of the time and moves between TMEM and registers the rest. Exponentials by polynomial on the FMA
+// units for one pair in eight made it slower (413 us): issue slots and latency, not the units, are short.
 // O is rescaled only when a row's maximum has grown by more than 2^8 since it last was: until then P is
 // taken against the old maximum, which fp32 sums and 16-bit P (at most 2^8) hold without loss, and O /
 // l is the same. P is rounded to 16 bits for the product (l adds it unrounded).
@@ -46,20 +50,31 @@ __device__ __forceinline__ int key_tiles(const AttnParams& p, int i0) {
   return (keys + kRows - 1) / kRows;
 }
 
+// The softmax warpgroups hold a row of 128 scores a thread and take the registers that the last
+// warpgroup, of the loader and the issuer, does not need: 2 x 128 = 208 + 48, 3 x 168 = 2 x 224 + 56.
+constexpr int kSoftRegs(int nq) { return nq == 1 ? 208 : 224; }
+constexpr int kRestRegs(int nq) { return nq == 1 ? 48 : 56; }
+
 template <typename T, int PANELS, int NQ, bool MASK>
-__global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1) attn_fwd_kernel(const __grid_constant__ FwdParams p) {
+__global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1) attn_fwd_kernel(const __grid_constant__ FwdParams p) {
   using L = FwdSmem<PANELS, NQ, MASK>;
   constexpr int STAGES = L::STAGES;
+  constexpr bool APART = PANELS == 1;  // P beside S: the next scores are computed while this tile is in its softmax
+  // With room for P beside S the query tiles' products need no common order, and a warp issues for each: the
+  // waits of one do not hold up the other (4 x 16 heads x 4096 x 64: 361 us, 381 with one issuer). Without it
+  // one issuer keeps them in turn; two would interleave their products and finish both late (dim 128: 563 us, 499).
+  constexpr int ISSUERS = APART ? NQ : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;
   uint8_t* sq = smem;
   uint8_t* skv = smem + NQ * L::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  uint64_t *q_full = bars, *full = q_full + NQ, *empty = full + STAGES, *s_full = empty + STAGES, *p_ready = s_full + NQ,
-           *o_full = p_ready + NQ, *done = o_full + NQ;
+  uint64_t *q_full = bars, *full = q_full + NQ, *empty = full + STAGES, *s_full = empty + STAGES, *s_free = s_full + NQ,
+           *p_ready = s_free + NQ, *pv_done = p_ready + NQ, *done = pv_done + NQ;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // the same in all lanes, and known to be: the roles below then run as uniform code
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   constexpr int LOADER = 4 * NQ, ISSUER = 4 * NQ + 1;
 
   unsigned x = blockIdx.x;
@@ -87,20 +102,21 @@ __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1) attn_fwd_kerne
     for (int w = 0; w < NQ; ++w) {
       mbar_init(q_full + w, 1);
       mbar_init(s_full + w, 1);
-      mbar_init(p_ready + w, 128);
-      mbar_init(o_full + w, 1);
+      mbar_init(s_free + w, 4);
+      mbar_init(p_ready + w, 4);
+      mbar_init(pv_done + w, 1);
     }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full + s, 1);
-      mbar_init(empty + s, 1);
+      mbar_init(empty + s, ISSUERS);
     }
-    mbar_init(done, 1);
+    mbar_init(done, ISSUERS);
     *abort_flag = 0;
     fence_mbar_init();
   }
   if (MASK)
     pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS), p.a.mask + b * p.a.mask_stride, most, p.a.kv_len, warp,
-                  NQ * 4 + 2, lane);
+                  NQ * 4 + 4, lane);
   if (warp == ISSUER) {
     tmem_alloc(tmem_slot, NQ == 2 ? 512 : 256);
     tmem_relinquish();
@@ -108,95 +124,126 @@ __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1) attn_fwd_kerne
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // columns: S of each query tile, O of each, and P of its own if there is room, else over S
   const uint32_t tmem = *tmem_slot;
+  auto s_at = [&](int w) { return tmem + w * 128; };
+  auto o_at = [&](int w) { return tmem + NQ * 128 + w * 64 * PANELS; };
+  auto p_at = [&](int w) { return APART ? tmem + NQ * 192 + w * 64 : tmem + w * 128; };
   const KeyBits bits{MASK ? reinterpret_cast<const uint4*>(smem + L::BITS) : nullptr};
 
-  if (warp == LOADER) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      const int j0 = bits.next(first, most);
-      for (int w = 0; w < NQ; ++w)
-        if (n[w] > j0) load_rows<PANELS>(sq + w * L::TILE, &p.mq, q_full + w, i0 + w * kRows, h, b);
-      for (int j = j0; ok && j < most; j = bits.next(j + 1, most)) {
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!(ok = mbar_wait(empty + s, ph ^ 1, abort_flag, p.a.status, ST_ATTN_LOAD))) break;
-          load_rows<PANELS>(skv + s * L::TILE, kv ? &p.mv : &p.mk, full + s, j * kRows, hk, b);
-          if (++s == STAGES) s = 0, ph ^= 1;
+  if (warp >= LOADER) {
+    regs_dec<kRestRegs(NQ)>();
+    if (warp == LOADER) {
+      if (lane == 0) {
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        const int j0 = bits.next(first, most);
+        for (int w = 0; w < NQ; ++w)
+          if (n[w] > j0) load_rows<PANELS>(sq + w * L::TILE, &p.mq, q_full + w, i0 + w * kRows, h, b);
+        for (int j = j0; ok && j < most; j = bits.next(j + 1, most)) {
+          for (int kv = 0; kv < 2; ++kv) {
+            if (!(ok = mbar_wait(empty + s, ph ^ 1, abort_flag, p.a.status, ST_ATTN_LOAD))) break;
+            load_rows<PANELS>(skv + s * L::TILE, kv ? &p.mv : &p.mk, full + s, j * kRows, hk, b);
+            if (++s == STAGES) s = 0, ph ^= 1;
+          }
         }
       }
-    }
-    __syncwarp();
-  } else if (warp == ISSUER) {
-    if (lane == 0) {
+      __syncwarp();
+    } else if (warp < ISSUER + ISSUERS) {
+      // The whole warp runs along, so that addresses and descriptors stay in uniform registers; one lane issues.
       const int ksteps = (p.a.head_dim + 15) / 16;
       const uint32_t idesc_s = make_idesc(128, 128, umma_format<T>(), 0, 0);
       const uint32_t idesc_o = make_idesc(128, ksteps * 16, umma_format<T>(), 0, 1);
-      auto s_at = [&](int w) { return tmem + w * 128; };
-      auto o_at = [&](int w) { return tmem + NQ * 128 + w * 64 * PANELS; };
-      // stage and phase of the next key tile; its values follow it
-      int s = 0;
-      uint32_t ph = 0, pph = 0;
+      const uint32_t qa = smem_u32(sq), kva = smem_u32(skv);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && mbar_wait(bar, parity, abort_flag, p.a.status, ST_ATTN_MMA);
+        ok = ok && warp_wait(bar, parity, abort_flag, p.a.status, ST_ATTN_MMA);
         tc_fence_after();
         return ok;
       };
-      auto scores = [&](int w, int stage) {
-        mma_scores(s_at(w), smem_u32(sq + w * L::TILE), smem_u32(skv + stage * L::TILE), idesc_s, ksteps);
+      auto scores = [&](int w, int s) {
+        mma_scores<PANELS>(s_at(w), qa + w * L::TILE, kva + s * L::TILE, idesc_s, ksteps);
         umma_commit(s_full + w);
       };
+      const int me = warp - ISSUER;
+      auto mine = [&](int w) { return ISSUERS == 1 || w == me; };
+      auto last = [&](int w) { return ISSUERS > 1 || w == NQ - 1; };  // of this issuer's: the stage is done with
+      // stage and phase of the tile's keys; its values lie in the next stage (the stage count is even)
+      int s = 0;
+      uint32_t ph = 0, pph = 0;
+      bool more = false;
       int j = bits.next(first, most);
       if (j < most && wait(full, 0)) {
-        for (int w = 0; w < NQ; ++w)
-          if (j < n[w] && wait(q_full + w, 0)) scores(w, 0);
-        umma_commit(empty);
+#pragma unroll
+        for (int w = 0; w < NQ; ++w) {
+          if (!mine(w) || (j < n[w] && !wait(q_full + w, 0))) continue;
+          if (elect_one()) {
+            if (j < n[w]) scores(w, 0);
+            if (last(w)) umma_commit(empty);
+          }
+          __syncwarp();
+        }
       }
-      uint32_t started = 0;
       while (ok && j < most) {
-        const int vs = s + 1;  // the stage count is even: a tile's keys and values lie side by side
+        const int vs = s + 1;
         const uint32_t vph = ph;
         s += 2;
         if (s == STAGES) s = 0, ph ^= 1;
         const int jn = bits.next(j + 1, most);
-        if (!wait(full + vs, vph)) break;
-        bool keys = false;
-        for (int w = 0; ok && w < NQ; ++w) {
-          if (j < n[w]) {
-            if (!wait(p_ready + w, pph)) break;
-            mma_probs(o_at(w), s_at(w), smem_u32(skv + vs * L::TILE), idesc_o, (started >> w) & 1, 32);
-            started |= 1u << w;
-            if (jn >= n[w]) umma_commit(o_full + w);
-          }
-          if (jn < n[w]) {
-            if (!keys && !wait(full + s, ph)) break;
-            keys = true;
-            scores(w, s);
+        if (APART && jn < most && wait(full + s, ph)) {
+#pragma unroll
+          for (int w = 0; w < NQ; ++w) {
+            if (!mine(w) || (jn < n[w] && !wait(s_free + w, pph))) continue;
+            if (elect_one()) {
+              if (jn < n[w]) scores(w, s);
+              if (last(w)) umma_commit(empty + s);
+            }
+            __syncwarp();
           }
         }
-        umma_commit(empty + vs);
-        if (jn < most) umma_commit(empty + s);
+        if (!ok || !wait(full + vs, vph)) break;
+#pragma unroll
+        for (int w = 0; w < NQ; ++w) {
+          if (!mine(w) || (j < n[w] && !wait(p_ready + w, pph))) continue;
+          if (elect_one()) {
+            if (j < n[w]) {
+              mma_probs<128, 128, 0>(o_at(w), p_at(w), kva + vs * L::TILE, idesc_o, more);
+              if (APART || jn >= n[w]) umma_commit(pv_done + w);
+            }
+            if (last(w)) umma_commit(empty + vs);
+          }
+          __syncwarp();
+          if (!APART && jn < most && wait(full + s, ph)) {
+            if (elect_one()) {
+              if (jn < n[w]) scores(w, s);
+              if (last(w)) umma_commit(empty + s);
+            }
+            __syncwarp();
+          }
+        }
+        more = true;
         pph ^= 1;
         j = jn;
       }
       // no product may be writing TMEM when it is released
-      umma_commit(done);
+      if (elect_one()) umma_commit(done);
+      __syncwarp();
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(done, 0))
         if (globaltimer_ns() - t0 > LSR_WAIT_TIMEOUT_NS) {
           set_status(p.a.status, ST_ATTN_DONE);
           break;
         }
+      __syncwarp();
     }
-    __syncwarp();
   } else {
+    regs_inc<kSoftRegs(NQ)>();
     const int w = warp / 4, r = (warp % 4) * 32 + lane, i = i0 + w * kRows + r;
     const int nw = NQ == 1 ? n[0] : (w ? n[NQ - 1] : n[0]);
     const bool idle = i0 + w * kRows + (warp % 4) * 32 >= p.a.q_len;  // none of the warp's rows exists
     const uint32_t at = (uint32_t)(warp % 4 * 32) << 16;
-    const uint32_t st = tmem + w * 128 + at, ot = tmem + NQ * 128 + w * 64 * PANELS + at;
+    const uint32_t st = s_at(w) + at, ot = o_at(w) + at, pt = p_at(w) + at;
     const float c = p.a.scale * kLog2e;
     // keys that the row sees, counted from the first
     const int sees = p.a.causal ? max(0, min(p.a.kv_len, i + 1 + p.a.kv_len - p.a.q_len)) : p.a.kv_len;
@@ -209,7 +256,6 @@ __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1) attn_fwd_kerne
     for (int j = bits.next(first, nw); j < nw; j = bits.next(j + 1, nw)) {
       if (!(ok = warp_wait(s_full + w, ph, abort_flag, p.a.status, ST_ATTN_SOFTMAX))) break;
       tc_fence_after();
-      ph ^= 1;
       uint4 word = make_uint4(~0u, ~0u, ~0u, ~0u);
       if (MASK) word = bits.bits[j];
       const bool holes = MASK && (word.x & word.y & word.z & word.w) != ~0u;
@@ -218,6 +264,7 @@ __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1) attn_fwd_kerne
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(st + q * 32, sr[q]);
         tmem_ld_wait();
+        if (APART) warp_arrive(s_free + w, lane);
         const int j0 = j * kRows;
         if (j0 + kRows > sees_all || j0 + kRows > p.a.kv_len || holes) {
 #pragma unroll
@@ -231,12 +278,15 @@ __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1) attn_fwd_kerne
         float top[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          top[q] = __uint_as_float(sr[q][0]);
+          top[q] = fmaxf(__uint_as_float(sr[q][0]), __uint_as_float(sr[q][1]));
 #pragma unroll
-          for (int e = 1; e < 32; ++e) top[q] = fmaxf(top[q], __uint_as_float(sr[q][e]));
+          for (int e = 2; e < 32; e += 2) top[q] = max3(top[q], __uint_as_float(sr[q][e]), __uint_as_float(sr[q][e + 1]));
         }
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         const bool grown = (mx - m) * c > kLazy;  // false for NaN, as of two minus infinities
+        // the product before has read P, and O may be rescaled (without P of its own the scores' wait said so)
+        if (APART && started && !(ok = warp_wait(pv_done + w, ph ^ 1, abort_flag, p.a.status, ST_ATTN_SOFTMAX))) break;
+        if (APART) tc_fence_after();
         if (__any_sync(0xffffffffu, grown)) {
           const float keep = grown ? ex2((m - mx) * c) : 1.f;
           if (grown) m = mx;
@@ -254,22 +304,33 @@ __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1) attn_fwd_kerne
           }
         }
         const float mc = m == -INFINITY ? 0.f : m * c;
-        float sum[4] = {};
+        const uint64_t c2 = pair(c, c), mc2 = pair(-mc, -mc);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           uint32_t pr[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float a0 = ex2(fmaf(__uint_as_float(sr[2 * q + e / 16][e % 16 * 2]), c, -mc));
-            const float a1 = ex2(fmaf(__uint_as_float(sr[2 * q + e / 16][e % 16 * 2 + 1]), c, -mc));
-            sum[e % 2 * 2] += a0;
-            sum[e % 2 * 2 + 1] += a1;
+            const uint32_t* v = &sr[2 * q + e / 16][e % 16 * 2];
+            const uint64_t x = fma2(pair(__uint_as_float(v[0]), __uint_as_float(v[1])), c2, mc2);
+            float a0, a1;
+            unpair(x, a0, a1);
+            a0 = ex2(a0);
+            a1 = ex2(a1);
+            sum[e % 2] = add2(sum[e % 2], pair(a0, a1));
             pr[e] = pack2<T>(a0, a1);
           }
-          tmem_st32(st + q * 32, pr);
+          tmem_st32(pt + q * 32, pr);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float l0, l1, l2, l3;
+        unpair(sum[0], l0, l1);
+        unpair(sum[1], l2, l3);
+        l += (l0 + l1) + (l2 + l3);
         tmem_st_wait();
+      } else if (APART) {
+        warp_arrive(s_free + w, lane);
+        // as the other warps, or its arrival for this tile could stand for theirs for the one before
+        if (started && !(ok = warp_wait(pv_done + w, ph ^ 1, abort_flag, p.a.status, ST_ATTN_SOFTMAX))) break;
       }
       started = true;
       if (holes) {  // a hidden key's probability is 0, but 0 times what its values hold need not be
@@ -286,10 +347,10 @@ __global__ void __launch_bounds__(NQ * 128 + 64, NQ == 1 ? 2 : 1) attn_fwd_kerne
       }
       vs += 2;
       if (vs > STAGES) vs = 1, vph ^= 1;
-      tc_fence_before();
-      mbar_arrive(p_ready + w);
+      ph ^= 1;
+      warp_arrive(p_ready + w, lane);
     }
-    if (ok && started) ok = warp_wait(o_full + w, 0, abort_flag, p.a.status, ST_ATTN_SOFTMAX);
+    if (ok && started) ok = warp_wait(pv_done + w, APART ? ph ^ 1 : 0, abort_flag, p.a.status, ST_ATTN_SOFTMAX);
     tc_fence_after();
     if (ok && !idle) {
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -389,7 +450,7 @@ int launch(FwdParams& p, cudaStream_t st) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess)
     return LSR_ERR_LAUNCH;
   ProfScope prof(PK_GEMM_OTHER, st);
-  kernel<<<(unsigned)blocks, NQ * 128 + 64, L::TOTAL, st>>>(p);
+  kernel<<<(unsigned)blocks, NQ * 128 + 128, L::TOTAL, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
 }
 

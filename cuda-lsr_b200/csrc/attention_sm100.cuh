@@ -20,6 +20,13 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Status codes of waits that ran out (lsr_device_status).
 enum : int { ST_ATTN_LOAD = 120, ST_ATTN_MMA = 121, ST_ATTN_SOFTMAX = 122, ST_ATTN_DONE = 123 };
 
+// One lane of the warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
+
 // D[tmem] (+)= A[tmem] * B[smem]: A is 128 lanes of 16-bit pairs, 8 columns per 16-deep step.
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -43,7 +50,25 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Give up or take registers, for a whole warpgroup (the block's total stays within what it was launched with).
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -51,10 +76,47 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // mbar_wait of a whole warp: one answer for all lanes, which the .aligned TMEM moves after it need.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
   const bool ok = mbar_wait(bar, parity, abort_flag, status, code);
   return __all_sync(0xffffffffu, ok);
+}
+
+// One arrival for a whole warp, after what its lanes did before (moves to and from TMEM included).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
 }
 
 // Two floats as one 32-bit pair of the 16-bit type, the first in the low half.
@@ -78,25 +140,28 @@ constexpr uint32_t umma_format<__nv_bfloat16>() { return 1; }
 template <>
 constexpr uint32_t umma_format<__half>() { return 0; }
 
-// D (128 x 128) = A B^T over the heads' entries: both tiles K-major, `steps` 16-entry steps.
-__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_smem, uint32_t b_smem, uint32_t idesc, int steps) {
-  const uint64_t a = smem_desc_sw128(a_smem, 16, 1024), b = smem_desc_sw128(b_smem, 16, 1024);
+// D (128 x N) = A B^T over the heads' entries: both tiles K-major, B from its row `b_row` on, `steps` 16-entry steps.
+template <int PANELS>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_smem, uint32_t b_smem, uint32_t idesc, int steps,
+                                           int b_row = 0) {
+  const uint64_t a = smem_desc_sw128(a_smem, 16, 1024), b = smem_desc_sw128(b_smem + b_row * 128, 16, 1024);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < 4 * PANELS; ++k) {
     if (k >= steps) break;
     const uint64_t off = (uint64_t)((k >> 2) * (kPanel >> 4) + (k & 3) * 2);
     umma_bf16(d, a + off, b + off, idesc, k > 0);
   }
 }
 
-// D (128 x entries) (+)= P B over the tile B's 128 rows: P in TMEM, the operand of the second 64 rows
-// `half` columns after that of the first.
+// D (128 x entries) (+)= P B over ROWS rows of the tile B, from `row` on: P in TMEM at p_tmem, the operands of
+// each PER rows APART columns after those of the ones before.
+template <int ROWS, int PER, int APART>
 __device__ __forceinline__ void mma_probs(uint32_t d, uint32_t p_tmem, uint32_t b_smem, uint32_t idesc, uint32_t accumulate,
-                                          int half) {
-  const uint64_t b = smem_desc_sw128(b_smem, kPanel, 1024);
+                                          int row = 0) {
+  const uint64_t b = smem_desc_sw128(b_smem + row * 128, kPanel, 1024);
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    umma_ts(d, p_tmem + (k >> 2) * half + (k & 3) * 8, b + (uint64_t)(k * (2048 >> 4)), idesc, accumulate || k > 0);
+  for (int k = 0; k < ROWS / 16; ++k)
+    umma_ts(d, p_tmem + (k * 16 / PER) * APART + (k * 16 % PER) / 2, b + (uint64_t)(k * (2048 >> 4)), idesc, accumulate || k > 0);
 }
 
 // One tile of [position][entry], panel by panel.

@@ -22,19 +22,21 @@ namespace {
 
 constexpr int GR_THREADS = 512;
 constexpr int GR_CHUNK = 1 << 15;  // entries
-constexpr int GR_TABLE = 1024;     // tensors per launch (30 bytes each of the 32764 bytes of kernel parameters)
+constexpr int GR_TABLE = 1024;     // tensors per launch at most (30 bytes each of the 32764 bytes of kernel parameters)
+constexpr int GR_SMALL = 96;       // a shorter list takes kernels with 3 KB of parameters instead of 30: less to copy per launch
 constexpr int GR_GRID = 592;       // blocks: 148 SMs x 4 blocks of 512 threads
 enum : int { NORM_MAX = 0, NORM_ONE = 1, NORM_TWO = 2 };
 
+template <int N>
 struct GradTable {
-  const void* in[GR_TABLE];
-  void* out[GR_TABLE];
-  long long numel[GR_TABLE];
-  int first[GR_TABLE];  // first chunk of the tensor
-  unsigned char tin[GR_TABLE], tout[GR_TABLE];
+  const void* in[N];
+  void* out[N];
+  long long numel[N];
+  int first[N];  // first chunk of the tensor
+  unsigned char tin[N], tout[N];
   int n, chunks;
 };
-static_assert(sizeof(GradTable) <= 32000, "kernel parameters");
+static_assert(sizeof(GradTable<GR_TABLE>) <= 32000, "kernel parameters");
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -89,7 +91,8 @@ __device__ __forceinline__ Acc<KIND> block_sum(Acc<KIND> a) {
 }
 
 // The tensor that holds chunk c.
-__device__ __forceinline__ int find_tensor(const GradTable& t, int c) {
+template <int N>
+__device__ __forceinline__ int find_tensor(const GradTable<N>& t, int c) {
   int lo = 0, hi = t.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -123,8 +126,8 @@ __device__ __forceinline__ void norm_chunk(const T* __restrict__ p, int n, Acc<K
   }
 }
 
-template <int KIND>
-__global__ void __launch_bounds__(GR_THREADS) grad_norm_kernel(const __grid_constant__ GradTable t,
+template <int KIND, int N>
+__global__ void __launch_bounds__(GR_THREADS) grad_norm_kernel(const __grid_constant__ GradTable<N> t,
                                                                Acc<KIND>* __restrict__ partial) {
   Acc<KIND> acc;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
@@ -190,8 +193,8 @@ __device__ __forceinline__ void scale_chunk_to(const TI* p, void* out, int tout,
 }
 
 // GIVEN: *norm is read (a norm of more tensors than these); else it is the partials' and is written.
-template <int KIND, bool GIVEN>
-__global__ void __launch_bounds__(GR_THREADS) grad_scale_kernel(const __grid_constant__ GradTable t,
+template <int KIND, bool GIVEN, int N>
+__global__ void __launch_bounds__(GR_THREADS) grad_scale_kernel(const __grid_constant__ GradTable<N> t,
                                                                 const Acc<KIND>* __restrict__ partial, int npartial,
                                                                 float max_norm, float* norm, int write_norm) {
   float total;
@@ -229,44 +232,56 @@ int check_list(const void* const* ptrs, const long long* numel, const int* dtype
 
 struct Span {
   uintptr_t lo, hi;
-  int tensor, out;
 };
 int span_order(const void* a, const void* b) {
   const Span *x = static_cast<const Span*>(a), *y = static_cast<const Span*>(b);
   return x->lo < y->lo ? -1 : x->lo > y->lo;
+}
+// By address; views of one buffer, the common list, come so.
+void sort_spans(Span* s, int n) {
+  for (int i = 1; i < n; ++i)
+    if (s[i].lo < s[i - 1].lo) {
+      qsort(s, n, sizeof(Span), span_order);
+      return;
+    }
 }
 
 // LSR_OK unless a written range overlaps another tensor's written or read range, or its own read
 // range other than exactly (in place): the blocks run in no order.
 int check_overlap(const void* const* in, void* const* out, const long long* numel, const int* tin, const int* tout,
                   int n) {
-  Span* s = static_cast<Span*>(malloc(sizeof(Span) * 2 * (size_t)n));
-  if (!s) return LSR_ERR_WORKSPACE;
-  int m = 0;
+  Span* w = static_cast<Span*>(malloc(sizeof(Span) * 2 * (size_t)n));
+  if (!w) return LSR_ERR_WORKSPACE;
+  Span* r = w + n;
+  int nw = 0, nr = 0;
   for (int i = 0; i < n; ++i) {
     if (!numel[i]) continue;
     const uintptr_t a = reinterpret_cast<uintptr_t>(in[i]), b = reinterpret_cast<uintptr_t>(out[i]);
-    s[m++] = Span{b, b + (uintptr_t)numel[i] * dtype_size(tout[i]), i, 1};
-    if (a != b || tin[i] != tout[i]) s[m++] = Span{a, a + (uintptr_t)numel[i] * dtype_size(tin[i]), i, 0};
+    w[nw++] = Span{b, b + (uintptr_t)numel[i] * dtype_size(tout[i])};
+    if (a != b || tin[i] != tout[i]) r[nr++] = Span{a, a + (uintptr_t)numel[i] * dtype_size(tin[i])};
   }
-  qsort(s, m, sizeof(Span), span_order);
-  uintptr_t any_end = 0, out_end = 0;  // ends of the ranges seen so far
+  sort_spans(w, nw);
+  sort_spans(r, nr);
   int rc = LSR_OK;
-  for (int i = 0; i < m && rc == LSR_OK; ++i) {
-    if (s[i].lo < out_end || (s[i].out && s[i].lo < any_end)) rc = LSR_ERR_ARG;
-    any_end = std::max(any_end, s[i].hi);
-    if (s[i].out) out_end = std::max(out_end, s[i].hi);
+  for (int i = 1; i < nw && rc == LSR_OK; ++i)
+    if (w[i].lo < w[i - 1].hi) rc = LSR_ERR_ARG;
+  // reads may overlap one another, so a written range is compared with the furthest end of those that begin before its own
+  uintptr_t read_end = 0;
+  for (int i = 0, k = 0; i < nw && rc == LSR_OK; ++i) {
+    for (; k < nr && r[k].lo < w[i].hi; ++k) read_end = std::max(read_end, r[k].hi);
+    if (read_end > w[i].lo) rc = LSR_ERR_ARG;
   }
-  free(s);
+  free(w);
   return rc;
 }
 
 // The next tensors of the list, from *i on, as one launch's table.
-void fill_table(GradTable& t, const void* const* in, void* const* out, const long long* numel, const int* tin,
+template <int N>
+void fill_table(GradTable<N>& t, const void* const* in, void* const* out, const long long* numel, const int* tin,
                 const int* tout, int n, int* i) {
   t.n = 0;
   t.chunks = 0;
-  for (; *i < n && t.n < GR_TABLE; ++*i) {
+  for (; *i < n && t.n < N; ++*i) {
     if (!numel[*i]) continue;
     const long long c = (numel[*i] + GR_CHUNK - 1) / GR_CHUNK;
     if (t.n && t.chunks + c > (1ll << 30)) break;
@@ -284,8 +299,8 @@ void fill_table(GradTable& t, const void* const* in, void* const* out, const lon
 size_t ws_bytes(int n) { return (size_t)(n / GR_TABLE + 2) * GR_GRID * sizeof(double); }
 
 // Partials of every table; *count receives their number.
-template <int KIND>
-int launch_partials(GradTable& t, const void* const* in, const long long* numel, const int* tin, int n,
+template <int KIND, int N>
+int launch_partials(GradTable<N>& t, const void* const* in, const long long* numel, const int* tin, int n,
                     Acc<KIND>* partial, int room, int* count, cudaStream_t st) {
   *count = 0;
   for (int i = 0; i < n;) {
@@ -294,34 +309,34 @@ int launch_partials(GradTable& t, const void* const* in, const long long* numel,
     const int grid = std::min(t.chunks, GR_GRID);
     if (*count + grid > room) return LSR_ERR_WORKSPACE;
     ProfScope prof(PK_EW_OTHER, st);
-    grad_norm_kernel<KIND><<<grid, GR_THREADS, 0, st>>>(t, partial + *count);
+    grad_norm_kernel<KIND, N><<<grid, GR_THREADS, 0, st>>>(t, partial + *count);
     if (cudaGetLastError() != cudaSuccess) return LSR_ERR_LAUNCH;
     *count += grid;
   }
   return LSR_OK;
 }
 
-template <int KIND>
-int norm_impl(const void* const* in, const long long* numel, const int* tin, int n, float* norm, void* ws, size_t bytes,
+template <int KIND, int N>
+int norm_table(const void* const* in, const long long* numel, const int* tin, int n, float* norm, void* ws, size_t bytes,
               cudaStream_t st) {
-  GradTable t;
+  GradTable<N> t;
   auto* partial = static_cast<Acc<KIND>*>(ws);
   int count = 0;
-  const int rc = launch_partials<KIND>(t, in, numel, tin, n, partial, (int)(bytes / sizeof(double)), &count, st);
+  const int rc = launch_partials<KIND, N>(t, in, numel, tin, n, partial, (int)(bytes / sizeof(double)), &count, st);
   if (rc != LSR_OK) return rc;
   ProfScope prof(PK_EW_OTHER, st);
   grad_norm_finish_kernel<KIND><<<1, GR_THREADS, 0, st>>>(partial, count, norm);
   return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
 }
 
-template <int KIND, bool GIVEN>
-int clip_impl(const void* const* in, void* const* out, const long long* numel, const int* tin, const int* tout, int n,
+template <int KIND, bool GIVEN, int N>
+int clip_table(const void* const* in, void* const* out, const long long* numel, const int* tin, const int* tout, int n,
               float max_norm, float* norm, void* ws, size_t bytes, cudaStream_t st) {
-  GradTable t;
+  GradTable<N> t;
   auto* partial = static_cast<Acc<KIND>*>(ws);
   int count = 0;
   if (!GIVEN) {
-    const int rc = launch_partials<KIND>(t, in, numel, tin, n, partial, (int)(bytes / sizeof(double)), &count, st);
+    const int rc = launch_partials<KIND, N>(t, in, numel, tin, n, partial, (int)(bytes / sizeof(double)), &count, st);
     if (rc != LSR_OK) return rc;
   }
   int first = 1;
@@ -330,11 +345,26 @@ int clip_impl(const void* const* in, void* const* out, const long long* numel, c
     if (!t.n && !first) break;
     ProfScope prof(PK_EW_OTHER, st);
     const int grid = std::max(1, std::min(t.chunks, GR_GRID));
-    grad_scale_kernel<KIND, GIVEN><<<grid, GR_THREADS, 0, st>>>(t, partial, count, max_norm, norm, first);
+    grad_scale_kernel<KIND, GIVEN, N><<<grid, GR_THREADS, 0, st>>>(t, partial, count, max_norm, norm, first);
     if (cudaGetLastError() != cudaSuccess) return LSR_ERR_LAUNCH;
     first = 0;
   }
   return LSR_OK;
+}
+
+template <int KIND>
+int norm_impl(const void* const* in, const long long* numel, const int* tin, int n, float* norm, void* ws, size_t bytes,
+              cudaStream_t st) {
+  return n <= GR_SMALL ? norm_table<KIND, GR_SMALL>(in, numel, tin, n, norm, ws, bytes, st)
+                       : norm_table<KIND, GR_TABLE>(in, numel, tin, n, norm, ws, bytes, st);
+}
+
+template <int KIND, bool GIVEN>
+int clip_impl(const void* const* in, void* const* out, const long long* numel, const int* tin, const int* tout, int n,
+              float max_norm, float* norm, void* ws, size_t bytes, cudaStream_t st) {
+  return n <= GR_SMALL
+             ? clip_table<KIND, GIVEN, GR_SMALL>(in, out, numel, tin, tout, n, max_norm, norm, ws, bytes, st)
+             : clip_table<KIND, GIVEN, GR_TABLE>(in, out, numel, tin, tout, n, max_norm, norm, ws, bytes, st);
 }
 
 }  // namespace

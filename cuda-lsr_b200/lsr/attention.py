@@ -6,8 +6,8 @@
 
 q is [batch, q_len, heads, dim], k and v [batch, kv_len, kv_heads, dim], heads a multiple of kv_heads
 (query head h reads key head h // (heads // kv_heads)), dim 1..128; fp32, bf16 or fp16, all alike. Any
-strides: entries of a head that are not contiguous are copied first, everything else is read in place
-(the three parts of one projection's output, or [batch, heads, length, dim] tensors transposed).
+strides: the three parts of one projection's output or [batch, heads, length, dim] tensors transposed are
+read in place; what is expanded, not on 16-byte boundaries or not contiguous within a head is copied first.
 ``causal`` lets query i see keys up to i + kv_len - q_len, so that the last query sees the last key.
 ``key_mask`` is bool [batch, kv_len], True = seen; what the masked keys hold does not matter. A query
 that sees no key has output 0, lse minus infinity and no gradient. lse is fp32 [batch, heads, q_len],
@@ -29,27 +29,28 @@ from . import _lib
 
 # lsr_attention_args (include/lsr.h): 8 ints, a float and its padding, 10 pointers, 25 strides
 _ARGS = struct.Struct("=8if4x10Q25q")
-_NONE = (0, 0, 0)
+_NO_GRADS = ((0,) * 4, (0,) * 12)
 
 
 def _check(q, k, v, key_mask):
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (liblsr has no CPU path)")
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be [batch, length, heads, dim]")
-    if q.dtype not in _lib.DTYPE_CODES:
-        raise ValueError(f"q must be fp32, bf16 or fp16 (got {q.dtype})")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"q, k and v must be of one type (got {q.dtype}, {k.dtype}, {v.dtype})")
-    if k.device != q.device or v.device != q.device:
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise ValueError("q, k and v must be CUDA tensors (liblsr has no CPU path)")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4:
+        raise ValueError("q, k and v must be [batch, length, heads, dim]")
+    dtype, device = q.dtype, q.get_device()
+    if dtype not in _lib.DTYPE_CODES:
+        raise ValueError(f"q must be fp32, bf16 or fp16 (got {dtype})")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"q, k and v must be of one type (got {dtype}, {k.dtype}, {v.dtype})")
+    if k.get_device() != device or v.get_device() != device:
         raise ValueError("q, k and v must be on the same CUDA device")
-    b, _, h, d = q.shape
-    if k.shape != v.shape:
-        raise ValueError(f"k and v must have one shape (got {tuple(k.shape)} and {tuple(v.shape)})")
-    _, n, hk, dk = k.shape
-    if k.shape[0] != b or dk != d:
-        raise ValueError(f"k is {tuple(k.shape)}: batch {b} and dim {d} are q's")
+    if v.shape != ks:
+        raise ValueError(f"k and v must have one shape (got {tuple(ks)} and {tuple(v.shape)})")
+    b, _, h, d = qs
+    bk, n, hk, dk = ks
+    if bk != b or dk != d:
+        raise ValueError(f"k is {tuple(ks)}: batch {b} and dim {d} are q's")
     if not 1 <= d <= 128:
         raise ValueError(f"dim must be 1 to 128 (got {d})")
     if hk < 1 or h < 1 or h % hk:
@@ -57,12 +58,20 @@ def _check(q, k, v, key_mask):
     if key_mask is not None:
         if key_mask.dtype != torch.bool or key_mask.shape != (b, n):
             raise ValueError(f"key_mask must be bool [{b}, {n}]")
-        if key_mask.device != q.device:
+        if key_mask.get_device() != device:
             raise ValueError("key_mask must be on q's device")
 
 
 def _read(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+    """t, or a copy where its strides or address keep it from the kernels that dim and type allow."""
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t
+    *strides, last = t.stride()
+    *sizes, d = t.shape
+    good = last == 1 or d == 1
+    if good and d % 8 == 0 and t.element_size() == 2:  # on the tensor cores, read by TMA
+        good = not t.data_ptr() & 15 and all(st % 8 == 0 and st > 0 for st, sz in zip(strides, sizes) if sz != 1)
+    return t if good else t.detach().clone(memory_format=torch.contiguous_format)
 
 
 def _mask(m: torch.Tensor | None) -> torch.Tensor | None:
@@ -70,15 +79,18 @@ def _mask(m: torch.Tensor | None) -> torch.Tensor | None:
 
 
 def _pack(q, k, v, key_mask, causal, scale, out, lse, dout=None, dq=None, dk=None, dv=None) -> bytes:
-    back = dout is not None
-    ptr = [q.data_ptr(), k.data_ptr(), v.data_ptr(), key_mask.data_ptr() if key_mask is not None else 0,
-           out.data_ptr(), lse.data_ptr()]
-    ptr += [dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()] if back else [0, 0, 0, 0]
-    strides = [s for t in (q, k, v, out) for s in t.stride()[:3]]
-    strides += [s for t in (dout, dq, dk, dv) for s in t.stride()[:3]] if back else [0] * 12
     b, n, h, d = q.shape
-    return _ARGS.pack(_lib.DTYPE_CODES[q.dtype], b, n, k.shape[1], h, k.shape[2], d, int(causal), scale, *ptr, *strides,
-                      key_mask.stride(0) if key_mask is not None else 0)
+    m, hk = k.shape[1:3]
+    own = n * h * d, h * d, d  # strides of a contiguous tensor of q's shape
+    back = _NO_GRADS
+    if dout is not None:
+        own_k = m * hk * d, hk * d, d
+        back = ((dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()), (*dout.stride()[:3], *own, *own_k, *own_k))
+    return _ARGS.pack(
+        _lib.DTYPE_CODES[q.dtype], b, n, m, h, hk, d, 1 if causal else 0, d ** -0.5 if scale is None else scale,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if key_mask is None else key_mask.data_ptr(), out.data_ptr(),
+        lse.data_ptr(), *back[0], *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *back[1],
+        0 if key_mask is None else key_mask.stride(0))
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
@@ -86,29 +98,23 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def _scale(scale, q) -> float:
-    return float(q.shape[3]) ** -0.5 if scale is None else float(scale)
-
-
-@torch.no_grad()
 def attention_forward(q, k, v, *, causal: bool = False, scale: float | None = None, key_mask=None):
     """(out, lse): the attention of q over k and v, and the log-sum-exp of each query's scores."""
     _check(q, k, v, key_mask)
     q, k, v, key_mask = _read(q), _read(k), _read(v), _mask(key_mask)
     b, n, h, d = q.shape
-    lib = _lib.load()
-    with _lib.on_device(q.device):
-        out = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
-        lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device)
-        args = _pack(q, k, v, key_mask, causal, _scale(scale, q), out, lse)
+    lib, dev = _lib.load(), q.device
+    with _lib.on_device(dev):
+        out = torch.empty((b, n, h, d), dtype=q.dtype, device=dev)
+        lse = torch.empty((b, h, n), dtype=torch.float32, device=dev)
+        args = _pack(q, k, v, key_mask, causal, scale, out, lse)
         nbytes = lib.lsr_attention_forward_workspace_bytes(args)
-        ws = _workspace(nbytes, q.device)
-        rc = lib.lsr_attention_forward(args, ws.data_ptr() if nbytes else None, nbytes, _lib.stream_handle(q.device))
+        ws = _workspace(nbytes, dev)
+        rc = lib.lsr_attention_forward(args, ws.data_ptr() if nbytes else None, nbytes, _lib.stream_handle(dev))
     _lib.check(rc, "lsr_attention_forward")
     return out, lse
 
 
-@torch.no_grad()
 def attention_backward(dout, q, k, v, out, lse, *, causal: bool = False, scale: float | None = None, key_mask=None):
     """(dq, dk, dv) from the output's gradient and what attention_forward returned for the same arguments."""
     _check(q, k, v, key_mask)
@@ -119,13 +125,14 @@ def attention_backward(dout, q, k, v, out, lse, *, causal: bool = False, scale: 
         raise ValueError("lse must be fp32 [batch, heads, q_len] on q's device")
     dout, q, k, v, out, key_mask = _read(dout), _read(q), _read(k), _read(v), _read(out), _mask(key_mask)
     lse = lse.contiguous()
-    lib = _lib.load()
-    with _lib.on_device(q.device):
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        args = _pack(q, k, v, key_mask, causal, _scale(scale, q), out, lse, dout, dq, dk, dv)
+    lib, dev, dtype = _lib.load(), q.device, q.dtype
+    with _lib.on_device(dev):
+        dq = torch.empty(q.shape, dtype=dtype, device=dev)
+        dk, dv = torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
+        args = _pack(q, k, v, key_mask, causal, scale, out, lse, dout, dq, dk, dv)
         nbytes = lib.lsr_attention_backward_workspace_bytes(args)
-        ws = _workspace(nbytes, q.device)
-        rc = lib.lsr_attention_backward(args, ws.data_ptr() if nbytes else None, nbytes, _lib.stream_handle(q.device))
+        ws = _workspace(nbytes, dev)
+        rc = lib.lsr_attention_backward(args, ws.data_ptr() if nbytes else None, nbytes, _lib.stream_handle(dev))
     _lib.check(rc, "lsr_attention_backward")
     return dq, dk, dv
 

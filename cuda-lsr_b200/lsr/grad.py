@@ -28,6 +28,17 @@ from . import _lib
 _KINDS = {math.inf: 0, 1.0: 1, 2.0: 2}
 
 
+# A model has hundreds of gradients: their properties are read by map over the unbound getters.
+_ptr_of, _numel_of, _size_of, _is_contiguous = (torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.size,
+                                                torch.Tensor.is_contiguous)
+_layout_of, _device_of, _dtype_of = (torch.Tensor.layout.__get__, torch.Tensor.device.__get__,
+                                     torch.Tensor.dtype.__get__)
+
+
+def _is_tensor(t) -> bool:
+    return isinstance(t, torch.Tensor)
+
+
 def _kind(norm_type) -> int:
     try:
         return _KINDS[float(norm_type)]
@@ -49,24 +60,22 @@ def _dense(t: torch.Tensor) -> bool:
 
 def _check_list(tensors, what: str) -> list[torch.Tensor]:
     ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    for t in ts:
-        if not isinstance(t, torch.Tensor):
-            raise ValueError(f"{what} must be tensors")
-        if t.layout != torch.strided:
-            raise ValueError(f"{what} must be dense tensors (got {t.layout})")
-    for dtype, device in {(t.dtype, t.device) for t in ts}:
-        if device.type != "cuda":
-            raise ValueError(f"{what} must be CUDA tensors (liblsr has no CPU path)")
-        if dtype not in _lib.DTYPE_CODES:
-            raise ValueError(f"{what} must be fp32, bf16 or fp16 (got {dtype})")
-        if device != ts[0].device:
-            raise ValueError(f"{what} must be on one device (got {device} and {ts[0].device})")
+    if not all(map(_is_tensor, ts)):
+        raise ValueError(f"{what} must be tensors")
+    layouts, devices, dtypes = set(map(_layout_of, ts)), set(map(_device_of, ts)), set(map(_dtype_of, ts))
+    if layouts - {torch.strided}:
+        raise ValueError(f"{what} must be dense tensors (got {layouts - {torch.strided}})")
+    if any(d.type != "cuda" for d in devices):
+        raise ValueError(f"{what} must be CUDA tensors (liblsr has no CPU path)")
+    if dtypes - _lib.DTYPE_CODES.keys():
+        raise ValueError(f"{what} must be fp32, bf16 or fp16 (got {dtypes - _lib.DTYPE_CODES.keys()})")
+    if len(devices) > 1:
+        raise ValueError(f"{what} must be on one device (got {devices})")
     return ts
 
 
 def _arrays(ts):
-    codes = _lib.DTYPE_CODES
-    return array("Q", [t.data_ptr() for t in ts]), array("i", [codes[t.dtype] for t in ts])
+    return array("Q", list(map(_ptr_of, ts))), array("i", [_lib.DTYPE_CODES[t] for t in map(_dtype_of, ts)])
 
 
 def _workspace(lib, count: int, device: torch.device) -> torch.Tensor:
@@ -78,6 +87,25 @@ def _address(a: array) -> int:
     return a.buffer_info()[0]
 
 
+def _flatten(ts, outs):
+    """(gradients, outputs, [(output, where its values are written first)]) that fill ranges of memory in one order."""
+    src, dst, back = [], [], []
+    for t, o in zip(ts, outs):
+        if _dense(t) and _dense(o) and t.stride() == o.stride():
+            src.append(t)
+            dst.append(o)
+            continue
+        if any(st == 0 and sz > 1 for st, sz in zip(o.stride(), o.shape)):
+            raise ValueError("an output's entries share memory (an expanded tensor): clip a copy of it")
+        src.append(t.contiguous())
+        if o.is_contiguous():
+            dst.append(o)
+        else:
+            dst.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
+            back.append((o, dst[-1]))
+    return src, dst, back
+
+
 @torch.no_grad()
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """The norm (1, 2 or inf) over every entry of every tensor: a 0-d fp32 tensor on their device."""
@@ -85,14 +113,15 @@ def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     ts = _check_list(tensors, "tensors")
     if not ts:
         return torch.zeros(())
-    ts = [t if _dense(t) else t.contiguous() for t in ts]
+    if not all(map(_is_contiguous, ts)):
+        ts = [t if _dense(t) else t.contiguous() for t in ts]
     dev = ts[0].device
     lib = _lib.load()
     with _lib.on_device(dev):
         norm = torch.empty((), dtype=torch.float32, device=dev)
         ws = _workspace(lib, len(ts), dev)
         ptrs, dtypes = _arrays(ts)
-        numel = array("q", [t.numel() for t in ts])
+        numel = array("q", list(map(_numel_of, ts)))
         rc = lib.lsr_grad_norm(_address(ptrs), _address(numel), _address(dtypes), len(ts), kind, norm.data_ptr(),
                                ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
     _lib.check(rc, "lsr_grad_norm")
@@ -115,7 +144,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
         raise ValueError(f"max_norm must be at least 0 (got {max_norm})")
     ts = _check_list(grads, "grads")
     outs = ts if out is None else _check_list(out, "out")
-    if len(outs) != len(ts) or any(o.shape != t.shape for o, t in zip(outs, ts)):
+    if outs is not ts and list(map(_size_of, outs)) != list(map(_size_of, ts)):
         raise ValueError("out must be one tensor of the same shape for each gradient")
     if not ts:
         return torch.zeros(()) if total_norm is None else total_norm
@@ -124,29 +153,16 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
         raise ValueError("out must be on the gradients' device")
     if total_norm is not None and (total_norm.dtype != torch.float32 or total_norm.device != dev or total_norm.numel() != 1):
         raise ValueError("total_norm must be one fp32 value on the gradients' device")
-    back = []  # (output, dense tensor to copy into it)
-    src, dst = [], []
-    for t, o in zip(ts, outs):
-        if t.is_contiguous() and o.is_contiguous():
-            src.append(t)
-            dst.append(o)
-        elif _dense(t) and _dense(o) and t.stride() == o.stride():
-            src.append(t)
-            dst.append(o)
-        else:
-            if any(st == 0 and sz > 1 for st, sz in zip(o.stride(), o.shape)):
-                raise ValueError("an output's entries share memory (an expanded tensor): clip a copy of it")
-            src.append(t.contiguous())
-            dst.append(o if o.is_contiguous() and o is not t else torch.empty(o.shape, dtype=o.dtype, device=dev))
-            if dst[-1] is not o:
-                back.append((o, dst[-1]))
+    src, dst, back = ts, outs, []
+    if not (all(map(_is_contiguous, ts)) and (outs is ts or all(map(_is_contiguous, outs)))):
+        src, dst, back = _flatten(ts, outs)
     lib = _lib.load()
     with _lib.on_device(dev):
         norm = torch.empty((), dtype=torch.float32, device=dev) if total_norm is None else total_norm
         ws = _workspace(lib, len(src), dev) if total_norm is None else None
         pin, tin = _arrays(src)
         pout, tout = _arrays(dst)
-        numel = array("q", [t.numel() for t in src])
+        numel = array("q", list(map(_numel_of, src)))
         rc = lib.lsr_grad_clip(_address(pin), _address(pout), _address(numel), _address(tin), _address(tout), len(src),
                                kind, max_norm, int(total_norm is not None), norm.data_ptr(),
                                ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
