@@ -47,6 +47,30 @@ __device__ __forceinline__ __nv_bfloat16 attn_from_f<__nv_bfloat16>(float x) { r
 template <>
 __device__ __forceinline__ __half attn_from_f<__half>(float x) { return __float2half_rn(x); }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // attention_general.cu: 32-bit arithmetic on the CUDA cores, any type, stride and alignment.
 int attention_forward_general(const AttnParams& p, int dtype, cudaStream_t st);
 int attention_backward_general(const AttnParams& p, int dtype, cudaStream_t st);

@@ -465,12 +465,12 @@ int query_tiles(const AttnParams& p) {
   return (long long)cdiv(p.q_len, 2 * kRows) * p.heads * p.batch >= device_sm_count() ? 2 : 1;
 }
 
-// Blocks that the key tiles of a block's queries are dealt to, when there are few queries.
+// Blocks that the key tiles of a block's queries are dealt to when there are few queries: as many as
+// the SMs have room for, with four tiles each at least, so that the join does not cost more than it saves.
 int split_count(const AttnParams& p) {
   const long long blocks = (long long)cdiv(p.q_len, query_tiles(p) * kRows) * p.heads * p.batch;
   const int tiles = cdiv(p.kv_len, kRows), room = 2 * device_sm_count();
-  if (blocks * 2 > room || tiles < 4) return 1;
-  return (int)std::min<long long>(std::min<long long>(room / blocks, tiles / 2), 64);
+  return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(room / blocks, tiles / 4), 64));
 }
 
 template <typename T>

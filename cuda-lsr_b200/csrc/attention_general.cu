@@ -6,119 +6,136 @@
 //   D_i  = do_i . o_i,  ds_ij = scale p_ij (do_i . v_j - D_i)
 //   dv_j = sum_i p_ij do_i,  dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i   (i over the group's heads too)
 //
-// Bound by the FFMA rate. A block of 256 threads owns 64 rows (queries in the forward pass and for
-// dq, keys for dk and dv) and passes over the other side in tiles of 64; each thread holds a 4 x 4
-// piece of the 64 x 64 scores and of the 64 x dim results, so a product reads two 16-byte vectors of
-// shared memory per 16 multiply-adds. Rows of a tile are dim + 4 floats apart: eight lanes that
-// read the same column of consecutive rows then fall on different banks. The forward pass keeps a
-// running maximum and sum per row; the backward pass computes p again from lse. dq and dk/dv come
-// from two passes, each of which sums in one fixed order: no atomics.
+// Bound by the FFMA rate and the shared-memory reads that feed it. A block of 8 warps is WR x G: WR sets of
+// 16 rows (queries in the forward pass and for dq, keys for dk and dv), and G shares of the columns of each
+// tile of the other side that the block passes over. The fewer rows there are, the more the columns are
+// shared, so that a short sequence or few key heads still fill the SMs; the shares' results are joined in
+// shared memory at the end, in order. A warp is 4 x 8 lanes; a lane holds 4 rows by CW / 8 columns of the
+// scores and 4 rows by dim / 8 entries of the results. Rows of a tile are dim + 4 floats apart, which puts
+// lanes that read consecutive rows on different banks. A row's maximum and sum are exchanged by shuffles
+// among 8 lanes. The forward pass keeps a running maximum
+// and sum per row; the backward pass computes p again from lse. dq and dk/dv come from two passes, each of
+// which sums in one fixed order: no atomics.
 // A masked key's row of k and v is taken as zeros, so that nothing in it reaches a result.
 #include "attention.cuh"
 
 namespace lsr {
 namespace {
 
-constexpr int AT = 64;        // rows and columns of a tile
-constexpr int ATHREADS = 256;
-constexpr int PLD = AT + 4;   // row of the score tile in shared memory
-
-// acc[r][c] += sum_d A[ty*4 + r][d] * B[tx + 16 c][d]   (both row-major, rows LD apart)
-template <int LD>
-__device__ __forceinline__ void mm_nt(const float* A, const float* B, int D, int ty, int tx, float (&acc)[4][4]) {
-#pragma unroll 4
-  for (int d = 0; d < D; d += 4) {
-    float4 a[4], b[4];
+// out[r][c] = sum_d A[4 r][d] * B[tx + 8 c][d]: A the first of the lane's rows, four apart, B a tile, rows LD
+// apart. Even and odd entries are summed apart, two to an instruction.
+template <int LD, int C>
+__device__ __forceinline__ void mm_nt(const float* A, const float* B, int tx, float (&out)[4][C]) {
+  uint64_t acc[4][C] = {};
+#pragma unroll 2
+  for (int d = 0; d < LD - 4; d += 4) {
+    ulonglong2 a[4], b[C];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4*>(A + (ty * 4 + r) * LD + d);
+    for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const ulonglong2*>(A + 4 * r * LD + d);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const float4*>(B + (tx + 16 * c) * LD + d);
+    for (int c = 0; c < C; ++c) b[c] = *reinterpret_cast<const ulonglong2*>(B + (tx + 8 * c) * LD + d);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        acc[r][c] = fmaf(a[r].x, b[c].x, acc[r][c]);
-        acc[r][c] = fmaf(a[r].y, b[c].y, acc[r][c]);
-        acc[r][c] = fmaf(a[r].z, b[c].z, acc[r][c]);
-        acc[r][c] = fmaf(a[r].w, b[c].w, acc[r][c]);
+      for (int c = 0; c < C; ++c) {
+        acc[r][c] = fma2(a[r].x, b[c].x, acc[r][c]);
+        acc[r][c] = fma2(a[r].y, b[c].y, acc[r][c]);
       }
   }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float even, odd;
+      unpair(acc[r][c], even, odd);
+      out[r][c] = even + odd;
+    }
 }
 
-// acc[ch][r][c] += sum_k P[ty*4 + r][k] * B[k][ch*64 + tx*4 + c]
-template <int LD, int CH>
-__device__ __forceinline__ void mm_nn(const float* P, const float* B, int ty, int tx, float (&acc)[CH][4][4]) {
+// A lane's part of a result: 4 rows by DIM / 8 entries, as pairs.
+template <int CH>
+using Sums = uint64_t[CH][4][2];
+
+// acc[ch][r][e] += sum_k P[4 r][k] * B[k][ch*32 + tx*4 + e] over the COLS rows of the tile B.
+template <int LD, int COLS, int CH>
+__device__ __forceinline__ void mm_nn(const float* P, const float* B, int tx, Sums<CH>& acc) {
 #pragma unroll 2
-  for (int k = 0; k < AT; k += 4) {
+  for (int k = 0; k < COLS; k += 4) {
     float4 a[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4*>(P + (ty * 4 + r) * PLD + k);
+    for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4*>(P + 4 * r * (COLS + 4) + k);
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-      for (int ch = 0; ch < CH; ++ch) {
-        const float4 b = *reinterpret_cast<const float4*>(B + (k + kk) * LD + ch * 64 + tx * 4);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float x = kk == 0 ? a[r].x : kk == 1 ? a[r].y : kk == 2 ? a[r].z : a[r].w;
-          acc[ch][r][0] = fmaf(x, b.x, acc[ch][r][0]);
-          acc[ch][r][1] = fmaf(x, b.y, acc[ch][r][1]);
-          acc[ch][r][2] = fmaf(x, b.z, acc[ch][r][2]);
-          acc[ch][r][3] = fmaf(x, b.w, acc[ch][r][3]);
-        }
-      }
-  }
-}
-
-// acc[ch][r][c] += sum_k P[k][ty*4 + r] * B[k][ch*64 + tx*4 + c]
-template <int LD, int CH>
-__device__ __forceinline__ void mm_tn(const float* P, const float* B, int ty, int tx, float (&acc)[CH][4][4]) {
-#pragma unroll 4
-  for (int k = 0; k < AT; ++k) {
-    const float4 a = *reinterpret_cast<const float4*>(P + k * PLD + ty * 4);
-#pragma unroll
-    for (int ch = 0; ch < CH; ++ch) {
-      const float4 b = *reinterpret_cast<const float4*>(B + k * LD + ch * 64 + tx * 4);
-      const float x[4] = {a.x, a.y, a.z, a.w};
+    for (int kk = 0; kk < 4; ++kk) {
+      uint64_t x[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        acc[ch][r][0] = fmaf(x[r], b.x, acc[ch][r][0]);
-        acc[ch][r][1] = fmaf(x[r], b.y, acc[ch][r][1]);
-        acc[ch][r][2] = fmaf(x[r], b.z, acc[ch][r][2]);
-        acc[ch][r][3] = fmaf(x[r], b.w, acc[ch][r][3]);
+        const float v = kk == 0 ? a[r].x : kk == 1 ? a[r].y : kk == 2 ? a[r].z : a[r].w;
+        x[r] = pair(v, v);
+      }
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) {
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(B + (k + kk) * LD + ch * 32 + tx * 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          acc[ch][r][0] = fma2(x[r], b.x, acc[ch][r][0]);
+          acc[ch][r][1] = fma2(x[r], b.y, acc[ch][r][1]);
+        }
       }
     }
   }
 }
 
-// Rows [row0, row0 + 64) of a [len][D] matrix with rows `stride` apart, zeros past len, past D and in
-// rows that `mask` hides.
+// `rows` rows from row0 on of a [len][D] matrix with rows `stride` apart, zeros past len, past D and in
+// rows that `mask` hides. vec (fp32 rows on 16-byte boundaries, D a multiple of 4): copied asynchronously, done
+// when the group that the caller commits is.
 template <typename T, int LD>
-__device__ __forceinline__ void load_tile(float* dst, const T* src, long long stride, int row0, int len, int D,
-                                          const unsigned char* mask) {
+__device__ __forceinline__ void load_tile(float* dst, int rows, const T* src, long long stride, int row0, int len, int D,
+                                          const unsigned char* mask, bool vec) {
   constexpr int W = LD - 4;
-  for (int i = threadIdx.x; i < AT * W; i += ATHREADS) {
-    const int r = i / W, d = i % W, g = row0 + r;
-    float x = 0.f;
-    if (g < len && d < D && (!mask || mask[g])) x = attn_to_f(src[(long long)g * stride + d]);
-    dst[r * LD + d] = x;
+  if (vec) {
+    for (int i = threadIdx.x; i < rows * (W / 4); i += blockDim.x) {
+      const int r = i / (W / 4), d = i % (W / 4) * 4, g = row0 + r;
+      const bool in = g < len && d < D && (!mask || mask[g]);
+      const float* from = reinterpret_cast<const float*>(src) + (in ? (long long)g * stride + d : 0);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * LD + d)), "l"(from), "r"(in ? 16 : 0)
+                   : "memory");
+    }
+  } else {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows * W; i += blockDim.x) {
+      const int r = i / W, d = i % W, g = row0 + r;
+      float x = 0.f;
+      if (g < len && d < D && (!mask || mask[g])) x = attn_to_f(src[(long long)g * stride + d]);
+      dst[r * LD + d] = x;
+    }
   }
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Wait until at most N of this thread's latest groups are on their way.
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
+// The lane's four rows of a result.
 template <typename T, int CH>
-__device__ __forceinline__ void store_tile(T* dst, long long stride, int row0, int len, int D, int ty, int tx,
-                                           const float (&acc)[CH][4][4], const float (&mul)[4]) {
+__device__ __forceinline__ void store_rows(T* dst, long long stride, int row0, int len, int D, int tx,
+                                           const Sums<CH>& acc, const float (&mul)[4]) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int g = row0 + ty * 4 + r;
+    const int g = row0 + 4 * r;
     if (g >= len) continue;
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
+    for (int ch = 0; ch < CH; ++ch) {
+      float x[4];
+      unpair(acc[ch][r][0], x[0], x[1]);
+      unpair(acc[ch][r][1], x[2], x[3]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int d = ch * 64 + tx * 4 + c;
-        if (d < D) dst[(long long)g * stride + d] = attn_from_f<T>(acc[ch][r][c] * mul[r]);
+        const int d = ch * 32 + tx * 4 + c;
+        if (d < D) dst[(long long)g * stride + d] = attn_from_f<T>(x[c] * mul[r]);
       }
+    }
   }
 }
 
@@ -134,82 +151,164 @@ struct Place {
   }
 };
 
-__device__ __forceinline__ bool sees(const AttnParams& p, const unsigned char* mask, int i, int j) {
-  return i < p.q_len && j < p.kv_len && (!p.causal || j <= i + (p.kv_len - p.q_len)) && (!mask || mask[j]);
-}
-
 // Keys that the rows before i_end can see, at most.
 __device__ __forceinline__ int key_end(const AttnParams& p, int i_end) {
   return p.causal ? max(0, min(p.kv_len, min(i_end, p.q_len) + (p.kv_len - p.q_len))) : p.kv_len;
 }
 
-template <typename T, int CH>
-__global__ void __launch_bounds__(ATHREADS) attn_fwd_general_kernel(const AttnParams p) {
-  constexpr int LD = CH * 64 + 4;
+// The G column shares of the block's rows, summed in order: every lane writes its part, then the block
+// adds and stores row by row.
+template <typename T, int DIM, int WR, int G>
+__device__ __forceinline__ void store_joined(float* room, T* dst, long long stride, int row0, int len, int D, int mine, int tx,
+                                             int share, const Sums<DIM / 32>& acc, const float (&mul)[4]) {
+  constexpr int ROWS = 16 * WR;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int ch = 0; ch < DIM / 32; ++ch)
+      *reinterpret_cast<ulonglong2*>(room + (share * ROWS + mine + 4 * r) * DIM + ch * 32 + tx * 4) =
+          make_ulonglong2(mul2(acc[ch][r][0], pair(mul[r], mul[r])), mul2(acc[ch][r][1], pair(mul[r], mul[r])));
+  __syncthreads();
+  for (int i = threadIdx.x; i < ROWS * DIM; i += blockDim.x) {
+    const int r = i / DIM, d = i % DIM;
+    if (row0 + r >= len || d >= D) continue;
+    float x = room[i];
+#pragma unroll
+    for (int g = 1; g < G; ++g) x += room[g * ROWS * DIM + i];
+    dst[(long long)(row0 + r) * stride + d] = attn_from_f<T>(x);
+  }
+}
+
+constexpr int GTHREADS = 256;
+
+template <int DIM, int WR, int G>
+struct FwdGeneral {
+  static constexpr int ROWS = 16 * WR, CW = G == 1 ? 64 : 32, COLS = CW * G, LD = DIM + 4;
+  static constexpr int FLOATS = ROWS * LD + 2 * COLS * LD + 8 * 16 * (CW + 4) + 2 * G * ROWS;
+  static constexpr int SMEM = FLOATS * 4;
+  static_assert(WR * G == 8 && G * ROWS * DIM <= ROWS * LD + 2 * COLS * LD, "the shares' results take the tiles' room");
+};
+
+template <typename T, int DIM, int WR, int G>
+__global__ void __launch_bounds__(GTHREADS, 1) attn_fwd_general_kernel(const AttnParams p, bool vec) {
+  using L = FwdGeneral<DIM, WR, G>;
+  constexpr int ROWS = L::ROWS, CW = L::CW, COLS = L::COLS, LD = L::LD, CH = DIM / 32, C = CW / 8;
   extern __shared__ float sm[];
-  float *Q = sm, *K = Q + AT * LD, *V = K + AT * LD, *P = V + AT * LD;
-  const Place at((p.q_len + AT - 1) / AT, p.heads);
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16, D = p.head_dim, i0 = at.tile * AT;
+  float *Q = sm, *K = Q + ROWS * LD, *V = K + COLS * LD, *PS = V + COLS * LD, *stat = PS + 8 * 16 * (CW + 4);
+  const Place at((p.q_len + ROWS - 1) / ROWS, p.heads);
+  const int warp = threadIdx.x / 32, ty = threadIdx.x % 32 / 8, tx = threadIdx.x % 8, D = p.head_dim;
+  const int i0 = at.tile * ROWS, mine = warp / G * 16 + ty;  // and every fourth row after it
+  const int share = warp % G, x0 = share * CW;               // the warp's columns of a tile
+  float* P = PS + (warp * 16 + ty) * (CW + 4);
   const unsigned char* mask = p.mask ? p.mask + at.b * p.mask_stride : nullptr;
   const T* k = attn_at<T>(p.k, p.sk, at.b, at.h / p.group);
   const T* v = attn_at<T>(p.v, p.sv, at.b, at.h / p.group);
-  load_tile<T, LD>(Q, attn_at<T>(p.q, p.sq, at.b, at.h), p.sq.s, i0, p.q_len, D, nullptr);
-  float o[CH][4][4] = {}, m[4], l[4] = {};
+  const int jend = key_end(p, i0 + ROWS), off = p.kv_len - p.q_len;
+  load_tile<T, LD>(Q, ROWS, attn_at<T>(p.q, p.sq, at.b, at.h), p.sq.s, i0, p.q_len, D, nullptr, vec);
+  if (jend > 0) load_tile<T, LD>(K, COLS, k, p.sk.s, 0, p.kv_len, D, mask, vec);
+  copies_commit();
+  if (jend > 0) load_tile<T, LD>(V, COLS, v, p.sv.s, 0, p.kv_len, D, mask, vec);
+  copies_commit();
+  Sums<CH> o = {};
+  float m[4], l[4] = {};
 #pragma unroll
   for (int r = 0; r < 4; ++r) m[r] = -INFINITY;
-  const int jend = key_end(p, i0 + AT);
-  for (int j0 = 0; j0 < jend; j0 += AT) {
+  for (int j0 = 0; j0 < jend; j0 += COLS) {
+    copies_wait<1>();
     __syncthreads();
-    load_tile<T, LD>(K, k, p.sk.s, j0, p.kv_len, D, mask);
-    load_tile<T, LD>(V, v, p.sv.s, j0, p.kv_len, D, mask);
+    float s[4][C];
+    mm_nt<LD, C>(Q + mine * LD, K + x0 * LD, tx, s);
     __syncthreads();
-    float s[4][4] = {};
-    mm_nt<LD>(Q, K, CH * 64, ty, tx, s);
+    // the next keys arrive during the softmax and the product with the values, the next values during the next scores
+    if (j0 + COLS < jend) load_tile<T, LD>(K, COLS, k, p.sk.s, j0 + COLS, p.kv_len, D, mask, vec);
+    copies_commit();
+    if (j0 + COLS > p.kv_len || mask || (p.causal && j0 + COLS - 1 > i0 + off)) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int j = j0 + x0 + tx + 8 * c;
+        const bool ok = j < p.kv_len && (!mask || mask[j]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!ok || (p.causal && j > i0 + mine + 4 * r + off)) s[r][c] = -INFINITY;
+      }
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[r][c] = sees(p, mask, i0 + ty * 4 + r, j0 + tx + 16 * c) ? s[r][c] * p.scale : -INFINITY;
+      for (int c = 0; c < C; ++c) {
+        // (not times the scale where hidden: it may be 0 or negative)
+        s[r][c] = s[r][c] == -INFINITY ? s[r][c] : s[r][c] * p.scale;
         top = fmaxf(top, s[r][c]);
       }
 #pragma unroll
-      for (int w = 8; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      for (int w = 4; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
       const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.f : mn;
       const float keep = expf(m[r] - base);
       float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < C; ++c) {
         const float e = expf(s[r][c] - base);
         sum += e;
-        P[(ty * 4 + r) * PLD + tx + 16 * c] = e;
+        P[4 * r * (CW + 4) + tx + 8 * c] = e;
       }
 #pragma unroll
-      for (int w = 8; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      for (int w = 4; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
       l[r] = l[r] * keep + sum;
       m[r] = mn;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[ch][r][c] *= keep;
+        for (int c = 0; c < 2; ++c) o[ch][r][c] = mul2(o[ch][r][c], pair(keep, keep));
     }
+    copies_wait<1>();
     __syncthreads();
-    mm_nn<LD, CH>(P, V, ty, tx, o);
+    mm_nn<LD, CW, CH>(P, V + x0 * LD, tx, o);
+    __syncthreads();
+    if (j0 + COLS < jend) load_tile<T, LD>(V, COLS, v, p.sv.s, j0 + COLS, p.kv_len, D, mask, vec);
+    copies_commit();
   }
-  float inv[4];
+  copies_wait<0>();
+  float mul[4];
+  if (G > 1) {  // the row's maximum and sum over all shares
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (tx == 0) {
+        stat[share * ROWS + mine + 4 * r] = m[r];
+        stat[(G + share) * ROWS + mine + 4 * r] = l[r];
+      }
+    __syncthreads();
+  }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    inv[r] = l[r] > 0.f || l[r] != l[r] ? 1.f / l[r] : 0.f;
-    const int g = i0 + ty * 4 + r;
-    if (tx == 0 && g < p.q_len) p.lse[((long long)at.b * p.heads + at.h) * p.q_len + g] = m[r] + logf(l[r]);
+    float top = m[r], total = l[r];
+    mul[r] = 1.f;
+    if (G > 1) {
+      const float* at_row = stat + mine + 4 * r;
+      top = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < G; ++g) top = fmaxf(top, at_row[g * ROWS]);
+      const float base = top == -INFINITY ? 0.f : top;
+      total = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) total += at_row[(G + g) * ROWS] * expf(at_row[g * ROWS] - base);
+      mul[r] = expf(m[r] - base);
+    }
+    mul[r] *= total > 0.f || total != total ? 1.f / total : 0.f;
+    const int g = i0 + mine + 4 * r;
+    if (tx == 0 && share == 0 && g < p.q_len)
+      p.lse[((long long)at.b * p.heads + at.h) * p.q_len + g] = top + logf(total);
   }
-  store_tile<T, CH>(attn_at<T>(p.out, p.so, at.b, at.h), p.so.s, i0, p.q_len, D, ty, tx, o, inv);
+  T* dst = attn_at<T>(p.out, p.so, at.b, at.h);
+  if constexpr (G == 1) store_rows<T, CH>(dst, p.so.s, i0 + mine, p.q_len, D, tx, o, mul);
+  else store_joined<T, DIM, WR, G>(sm, dst, p.so.s, i0, p.q_len, D, mine, tx, share, o, mul);
 }
 
 // delta[row] = dout . out, one warp per row.
 template <typename T>
-__global__ void __launch_bounds__(ATHREADS) attn_delta_kernel(const AttnParams p) {
-  const long long row = (long long)blockIdx.x * (ATHREADS / 32) + threadIdx.x / 32;
+__global__ void __launch_bounds__(256) attn_delta_kernel(const AttnParams p) {
+  const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
   if (row >= (long long)p.batch * p.heads * p.q_len) return;
   const int i = (int)(row % p.q_len), h = (int)(row / p.q_len % p.heads), b = (int)(row / p.q_len / p.heads);
   const T* o = attn_at<T>(p.out, p.so, b, h) + i * p.so.s;
@@ -221,141 +320,243 @@ __global__ void __launch_bounds__(ATHREADS) attn_delta_kernel(const AttnParams p
   if (threadIdx.x % 32 == 0) p.delta[row] = s;
 }
 
-// exp(s - lse), 0 where i does not see j (a row that sees nothing has lse = minus infinity).
-__device__ __forceinline__ float prob(const AttnParams& p, const unsigned char* mask, int i, int j, float s, float lse) {
-  return sees(p, mask, i, j) ? expf(s * p.scale - lse) : 0.f;
-}
+template <int DIM, int WR, int G, bool KEYS>
+struct BwdGeneral {
+  static constexpr int ROWS = 16 * WR, CW = 32, COLS = CW * G, LD = DIM + 4;
+  static constexpr int BUFS = G <= 2 ? 2 : 1;  // of the first operand's tile: the next one arrives during the step
+  static constexpr int FLOATS = 2 * ROWS * LD + (BUFS + 1) * COLS * LD + (KEYS ? 2 : 1) * 8 * 16 * (CW + 4) + BUFS * 2 * COLS;
+  static constexpr int SMEM = FLOATS * 4;
+  static_assert(WR * G == 8 && G * ROWS * DIM <= FLOATS, "the shares' results take the tiles' room");
+};
 
-template <typename T, int CH>
-__global__ void __launch_bounds__(ATHREADS) attn_dq_general_kernel(const AttnParams p) {
-  constexpr int LD = CH * 64 + 4;
+// KEYS: the rows are keys and the columns queries of every head of the group (dv and dk); else rows are
+// queries and columns keys (dq).
+template <typename T, int DIM, int WR, int G, bool KEYS>
+__global__ void __launch_bounds__(GTHREADS, 1) attn_bwd_general_kernel(const AttnParams p, bool vec) {
+  using L = BwdGeneral<DIM, WR, G, KEYS>;
+  constexpr int ROWS = L::ROWS, CW = L::CW, COLS = L::COLS, LD = L::LD, CH = DIM / 32, C = CW / 8, BUFS = L::BUFS;
   extern __shared__ float sm[];
-  float *Q = sm, *DO = Q + AT * LD, *K = DO + AT * LD, *V = K + AT * LD, *P = V + AT * LD;
-  const Place at((p.q_len + AT - 1) / AT, p.heads);
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16, D = p.head_dim, i0 = at.tile * AT;
+  float *R1 = sm, *R2 = R1 + ROWS * LD, *X1 = R2 + ROWS * LD, *X2 = X1 + BUFS * COLS * LD, *SS = X2 + COLS * LD;
+  float *PS = SS + 8 * 16 * (CW + 4), *stat = KEYS ? PS + 8 * 16 * (CW + 4) : PS;  // PS: only KEYS multiplies it
+  const int rows_len = KEYS ? p.kv_len : p.q_len, cols_len = KEYS ? p.q_len : p.kv_len;
+  const Place at((rows_len + ROWS - 1) / ROWS, KEYS ? p.kv_heads : p.heads);
+  const int warp = threadIdx.x / 32, ty = threadIdx.x % 32 / 8, tx = threadIdx.x % 8, D = p.head_dim;
+  const int row0 = at.tile * ROWS, mine = warp / G * 16 + ty;  // and every fourth row after it
+  const int share = warp % G, x0 = share * CW;                 // the warp's columns of a tile
+  float *P = PS + (warp * 16 + ty) * (CW + 4), *S = SS + (warp * 16 + ty) * (CW + 4);
+  const int hk = KEYS ? at.h : at.h / p.group;
   const unsigned char* mask = p.mask ? p.mask + at.b * p.mask_stride : nullptr;
-  const T* k = attn_at<T>(p.k, p.sk, at.b, at.h / p.group);
-  const T* v = attn_at<T>(p.v, p.sv, at.b, at.h / p.group);
-  load_tile<T, LD>(Q, attn_at<T>(p.q, p.sq, at.b, at.h), p.sq.s, i0, p.q_len, D, nullptr);
-  load_tile<T, LD>(DO, attn_at<T>(p.dout, p.sdo, at.b, at.h), p.sdo.s, i0, p.q_len, D, nullptr);
-  float lse[4], delta[4], acc[CH][4][4] = {}, mul[4];
+  const T *k = attn_at<T>(p.k, p.sk, at.b, hk), *v = attn_at<T>(p.v, p.sv, at.b, hk);
+  const int off = p.kv_len - p.q_len;
+  float lse[4], delta[4];
+  if (KEYS) {
+    load_tile<T, LD>(R1, ROWS, k, p.sk.s, row0, p.kv_len, D, mask, vec);
+    load_tile<T, LD>(R2, ROWS, v, p.sv.s, row0, p.kv_len, D, mask, vec);
+  } else {
+    load_tile<T, LD>(R1, ROWS, attn_at<T>(p.q, p.sq, at.b, at.h), p.sq.s, row0, p.q_len, D, nullptr, vec);
+    load_tile<T, LD>(R2, ROWS, attn_at<T>(p.dout, p.sdo, at.b, at.h), p.sdo.s, row0, p.q_len, D, nullptr, vec);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int g = i0 + ty * 4 + r;
-    const long long row = ((long long)at.b * p.heads + at.h) * p.q_len + g;
-    lse[r] = g < p.q_len ? p.lse[row] : 0.f;
-    delta[r] = g < p.q_len ? p.delta[row] : 0.f;
-    mul[r] = p.scale;
-  }
-  const int jend = key_end(p, i0 + AT);
-  for (int j0 = 0; j0 < jend; j0 += AT) {
-    __syncthreads();
-    load_tile<T, LD>(K, k, p.sk.s, j0, p.kv_len, D, mask);
-    load_tile<T, LD>(V, v, p.sv.s, j0, p.kv_len, D, mask);
-    __syncthreads();
-    float s[4][4] = {}, dp[4][4] = {};
-    mm_nt<LD>(Q, K, CH * 64, ty, tx, s);
-    mm_nt<LD>(DO, V, CH * 64, ty, tx, dp);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        P[(ty * 4 + r) * PLD + tx + 16 * c] =
-            prob(p, mask, i0 + ty * 4 + r, j0 + tx + 16 * c, s[r][c], lse[r]) * (dp[r][c] - delta[r]);
-    __syncthreads();
-    mm_nn<LD, CH>(P, K, ty, tx, acc);
-  }
-  store_tile<T, CH>(attn_at<T>(p.dq, p.sdq, at.b, at.h), p.sdq.s, i0, p.q_len, D, ty, tx, acc, mul);
-}
-
-template <typename T, int CH>
-__global__ void __launch_bounds__(ATHREADS) attn_dkv_general_kernel(const AttnParams p) {
-  constexpr int LD = CH * 64 + 4;
-  extern __shared__ float sm[];
-  float *K = sm, *V = K + AT * LD, *Q = V + AT * LD, *DO = Q + AT * LD, *P = DO + AT * LD, *S = P + AT * PLD;
-  const Place at((p.kv_len + AT - 1) / AT, p.kv_heads);
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16, D = p.head_dim, j0 = at.tile * AT;
-  const unsigned char* mask = p.mask ? p.mask + at.b * p.mask_stride : nullptr;
-  load_tile<T, LD>(K, attn_at<T>(p.k, p.sk, at.b, at.h), p.sk.s, j0, p.kv_len, D, mask);
-  load_tile<T, LD>(V, attn_at<T>(p.v, p.sv, at.b, at.h), p.sv.s, j0, p.kv_len, D, mask);
-  float dk[CH][4][4] = {}, dv[CH][4][4] = {};
-  const int first = p.causal ? max(0, j0 - (p.kv_len - p.q_len)) / AT * AT : 0;  // rows before it see none of these keys
-  for (int h = at.h * p.group; h < (at.h + 1) * p.group; ++h) {
-    const T* q = attn_at<T>(p.q, p.sq, at.b, h);
-    const T* dout = attn_at<T>(p.dout, p.sdo, at.b, h);
-    const long long row = ((long long)at.b * p.heads + h) * p.q_len;
-    for (int i0 = first; i0 < p.q_len; i0 += AT) {
-      __syncthreads();
-      load_tile<T, LD>(Q, q, p.sq.s, i0, p.q_len, D, nullptr);
-      load_tile<T, LD>(DO, dout, p.sdo.s, i0, p.q_len, D, nullptr);
-      __syncthreads();
-      float s[4][4] = {}, dp[4][4] = {};
-      mm_nt<LD>(Q, K, CH * 64, ty, tx, s);
-      mm_nt<LD>(DO, V, CH * 64, ty, tx, dp);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = i0 + ty * 4 + r;
-        const float lse = i < p.q_len ? p.lse[row + i] : 0.f, delta = i < p.q_len ? p.delta[row + i] : 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float e = prob(p, mask, i, j0 + tx + 16 * c, s[r][c], lse);
-          P[(ty * 4 + r) * PLD + tx + 16 * c] = e;
-          S[(ty * 4 + r) * PLD + tx + 16 * c] = e * (dp[r][c] - delta);
-        }
-      }
-      __syncthreads();
-      mm_tn<LD, CH>(P, DO, ty, tx, dv);
-      mm_tn<LD, CH>(S, Q, ty, tx, dk);
+    for (int r = 0; r < 4; ++r) {
+      const int g = row0 + mine + 4 * r;
+      const long long row = ((long long)at.b * p.heads + at.h) * p.q_len + g;
+      lse[r] = g < p.q_len ? p.lse[row] : 0.f;
+      delta[r] = g < p.q_len ? p.delta[row] : 0.f;
     }
   }
-  const float one[4] = {1.f, 1.f, 1.f, 1.f}, sc[4] = {p.scale, p.scale, p.scale, p.scale};
-  store_tile<T, CH>(attn_at<T>(p.dv, p.sdv, at.b, at.h), p.sdv.s, j0, p.kv_len, D, ty, tx, dv, one);
-  store_tile<T, CH>(attn_at<T>(p.dk, p.sdk, at.b, at.h), p.sdk.s, j0, p.kv_len, D, ty, tx, dk, sc);
+  Sums<KEYS ? CH : 1> acc1 = {};
+  Sums<CH> acc2 = {};
+  // queries before `first` see none of the block's keys; keys from `end` on are seen by none of its queries
+  const int first = KEYS && p.causal ? max(0, row0 - off) / CW * CW : 0;
+  const int end = KEYS ? cols_len : key_end(p, row0 + ROWS);
+  const int tiles = max(0, (end - first + COLS - 1) / COLS), steps = KEYS ? tiles * p.group : tiles;
+  // the tile that step t passes over, as the first operand (q or k; with the queries' statistics) and the second (dout or v)
+  auto load1 = [&](int t) {
+    float* dst = X1 + t % BUFS * COLS * LD;
+    if (KEYS) {
+      const int h = at.h * p.group + t / tiles, c0 = first + t % tiles * COLS;
+      load_tile<T, LD>(dst, COLS, attn_at<T>(p.q, p.sq, at.b, h), p.sq.s, c0, p.q_len, D, nullptr, vec);
+      for (int x = threadIdx.x; x < COLS; x += GTHREADS) {
+        const int i = c0 + x;
+        const long long row = ((long long)at.b * p.heads + h) * p.q_len + i;
+        stat[t % BUFS * 2 * COLS + x] = i < p.q_len ? p.lse[row] : 0.f;
+        stat[t % BUFS * 2 * COLS + COLS + x] = i < p.q_len ? p.delta[row] : 0.f;
+      }
+    } else {
+      load_tile<T, LD>(dst, COLS, k, p.sk.s, t * COLS, p.kv_len, D, mask, vec);
+    }
+  };
+  auto load2 = [&](int t) {
+    if (KEYS)
+      load_tile<T, LD>(X2, COLS, attn_at<T>(p.dout, p.sdo, at.b, at.h * p.group + t / tiles), p.sdo.s, first + t % tiles * COLS,
+                       p.q_len, D, nullptr, vec);
+    else load_tile<T, LD>(X2, COLS, v, p.sv.s, t * COLS, p.kv_len, D, mask, vec);
+  };
+  if (steps > 0) load1(0);
+  copies_commit();
+  if (steps > 0) load2(0);
+  copies_commit();
+  for (int t = 0; t < steps; ++t) {
+    const float* x1 = X1 + (t % BUFS * COLS + x0) * LD;
+    const float* st = stat + t % BUFS * 2 * COLS + x0;
+    const int c0 = first + (KEYS ? t % tiles : t) * COLS + x0;
+    if (BUFS == 2 && t + 1 < steps) load1(t + 1);
+    if (BUFS == 2) copies_commit();
+    copies_wait<BUFS>();
+    __syncthreads();
+    float s[4][C], dp[4][C];
+    mm_nt<LD, C>(R1 + mine * LD, x1, tx, s);
+    copies_wait<BUFS - 1>();
+    __syncthreads();
+    mm_nt<LD, C>(R2 + mine * LD, X2 + x0 * LD, tx, dp);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int x = c0 + tx + 8 * c;
+      const bool in = x < cols_len && (KEYS || !mask || mask[x]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int a = row0 + mine + 4 * r;
+        const float ls = KEYS ? st[tx + 8 * c] : lse[r], dl = KEYS ? st[COLS + tx + 8 * c] : delta[r];
+        // 0 where i does not see j (a row that sees nothing has lse = minus infinity); masked rows are left out at the end
+        const bool ok = in && (!p.causal || (KEYS ? a <= x + off : x <= a + off));
+        const float e = ok ? expf(s[r][c] * p.scale - ls) : 0.f;
+        if (KEYS) P[4 * r * (CW + 4) + tx + 8 * c] = e;
+        S[4 * r * (CW + 4) + tx + 8 * c] = ok ? e * (dp[r][c] - dl) : 0.f;
+      }
+    }
+    __syncwarp();  // the warp's rows of P and S are its own
+    if constexpr (KEYS) mm_nn<LD, CW, CH>(P, X2 + x0 * LD, tx, acc1);
+    __syncthreads();
+    if (t + 1 < steps) load2(t + 1);
+    copies_commit();
+    mm_nn<LD, CW, CH>(S, x1, tx, acc2);
+    __syncthreads();
+    if (BUFS == 1) {
+      if (t + 1 < steps) load1(t + 1);
+      copies_commit();
+      copies_commit();  // an empty group, so that the wait for all but one covers both operands
+    }
+  }
+  copies_wait<0>();
+  float one[4], sc[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int a = row0 + mine + 4 * r;
+    const bool hidden = KEYS && mask && a < p.kv_len && !mask[a];  // a masked key has no gradient
+    if (KEYS && hidden) {
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) acc1[KEYS ? ch : 0][r][c] = acc2[ch][r][c] = 0;
+    }
+    one[r] = 1.f;
+    sc[r] = p.scale;
+  }
+  auto store = [&](void* base, const AttnStride& sd, const Sums<CH>& acc, const float(&mul)[4]) {
+    T* dst = attn_at<T>(base, sd, at.b, at.h);
+    if constexpr (G == 1) store_rows<T, CH>(dst, sd.s, row0 + mine, rows_len, D, tx, acc, mul);
+    else store_joined<T, DIM, WR, G>(sm, dst, sd.s, row0, rows_len, D, mine, tx, share, acc, mul);
+  };
+  if constexpr (KEYS) {
+    store(p.dv, p.sdv, acc1, one);
+    store(p.dk, p.sdk, acc2, sc);
+  } else {
+    store(p.dq, p.sdq, acc2, sc);
+  }
 }
 
-template <typename K>
-int launch(K kernel, const AttnParams& p, long long blocks, int smem, cudaStream_t st) {
+// Whether fp32 rows can be read as 16-byte vectors.
+bool vec_ok(const void* base, const AttnStride& s, int batch, int heads, int len, int dim) {
+  const auto fits = [](long long st, int size) { return size <= 1 || st % 4 == 0; };
+  return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && dim % 4 == 0 && fits(s.b, batch) && fits(s.s, len) && fits(s.h, heads);
+}
+
+template <typename K, typename... A>
+int launch(K kernel, long long blocks, int threads, int smem, cudaStream_t st, A... args) {
   if (blocks == 0) return LSR_OK;
   if (blocks > 0x7fffffffll) return LSR_ERR_SHAPE;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return LSR_ERR_LAUNCH;
   ProfScope prof(PK_GEMM_OTHER, st);
-  kernel<<<(unsigned)blocks, ATHREADS, smem, st>>>(p);
+  kernel<<<(unsigned)blocks, threads, smem, st>>>(args...);
   return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
 }
 
-template <typename T, int CH>
-int forward(const AttnParams& p, cudaStream_t st) {
-  const int tile = AT * (CH * 64 + 4) * 4, score = AT * PLD * 4;
-  return launch(attn_fwd_general_kernel<T, CH>, p, (long long)cdiv(p.q_len, AT) * p.heads * p.batch, 3 * tile + score, st);
+// Sets of 16 rows per block: the most whose blocks still fill the SMs.
+int row_sets(long long rows, long long heads, int least) {
+  for (int w = 8; w > least; w /= 2)
+    if ((rows + 16 * w - 1) / (16 * w) * heads >= device_sm_count()) return w;
+  return least;
 }
 
-template <typename T, int CH>
-int backward(const AttnParams& p, cudaStream_t st) {
-  const int tile = AT * (CH * 64 + 4) * 4, score = AT * PLD * 4;
+template <typename T, int DIM, int WR>
+int forward_w(const AttnParams& p, bool vec, cudaStream_t st) {
+  using L = FwdGeneral<DIM, WR, 8 / WR>;
+  static_assert(L::SMEM <= 232448, "shared memory budget exceeded");
+  return launch(attn_fwd_general_kernel<T, DIM, WR, 8 / WR>, (long long)cdiv(p.q_len, L::ROWS) * p.heads * p.batch, GTHREADS,
+                L::SMEM, st, p, vec);
+}
+
+template <typename T, int DIM, int WR, bool KEYS>
+int backward_w(const AttnParams& p, bool vec, cudaStream_t st) {
+  using L = BwdGeneral<DIM, WR, 8 / WR, KEYS>;
+  static_assert(L::SMEM <= 232448, "shared memory budget exceeded");
+  return launch(attn_bwd_general_kernel<T, DIM, WR, 8 / WR, KEYS>,
+                (long long)cdiv(KEYS ? p.kv_len : p.q_len, L::ROWS) * (KEYS ? p.kv_heads : p.heads) * p.batch, GTHREADS,
+                L::SMEM, st, p, vec);
+}
+
+constexpr int least_sets(int dim) { return dim == 64 ? 1 : 2; }  // eight shares of 128 wide tiles do not fit
+
+template <typename T, int DIM>
+int forward(const AttnParams& p, bool vec, cudaStream_t st) {
+  switch (row_sets(p.q_len, (long long)p.heads * p.batch, least_sets(DIM))) {
+    case 8: return forward_w<T, DIM, 8>(p, vec, st);
+    case 4: return forward_w<T, DIM, 4>(p, vec, st);
+    case 2: return forward_w<T, DIM, 2>(p, vec, st);
+    default: return forward_w<T, DIM, least_sets(DIM)>(p, vec, st);
+  }
+}
+
+template <typename T, int DIM, bool KEYS>
+int gradients(const AttnParams& p, bool vec, cudaStream_t st) {
+  switch (row_sets(KEYS ? p.kv_len : p.q_len, (long long)(KEYS ? p.kv_heads : p.heads) * p.batch, least_sets(DIM))) {
+    case 8: return backward_w<T, DIM, 8, KEYS>(p, vec, st);
+    case 4: return backward_w<T, DIM, 4, KEYS>(p, vec, st);
+    case 2: return backward_w<T, DIM, 2, KEYS>(p, vec, st);
+    default: return backward_w<T, DIM, least_sets(DIM), KEYS>(p, vec, st);
+  }
+}
+
+template <typename T, int DIM>
+int backward(const AttnParams& p, bool vec, cudaStream_t st) {
   const long long rows = (long long)p.batch * p.heads * p.q_len;
-  int rc = launch(attn_delta_kernel<T>, p, (rows + ATHREADS / 32 - 1) / (ATHREADS / 32), 0, st);
-  if (rc != LSR_OK) return rc;
-  rc = launch(attn_dkv_general_kernel<T, CH>, p, (long long)cdiv(p.kv_len, AT) * p.kv_heads * p.batch,
-              4 * tile + 2 * score, st);
-  if (rc != LSR_OK) return rc;
-  return launch(attn_dq_general_kernel<T, CH>, p, (long long)cdiv(p.q_len, AT) * p.heads * p.batch, 4 * tile + score, st);
+  int rc = launch(attn_delta_kernel<T>, (rows + 7) / 8, 256, 0, st, p);
+  if (rc == LSR_OK) rc = gradients<T, DIM, true>(p, vec, st);
+  return rc == LSR_OK ? gradients<T, DIM, false>(p, vec, st) : rc;
 }
 
 }  // namespace
 
 int attention_forward_general(const AttnParams& p, int dtype, cudaStream_t st) {
   const bool wide = p.head_dim > 64;
-  if (dtype == LSR_DTYPE_F32) return wide ? forward<float, 2>(p, st) : forward<float, 1>(p, st);
-  if (dtype == LSR_DTYPE_BF16) return wide ? forward<__nv_bfloat16, 2>(p, st) : forward<__nv_bfloat16, 1>(p, st);
-  return wide ? forward<__half, 2>(p, st) : forward<__half, 1>(p, st);
+  const bool vec = dtype == LSR_DTYPE_F32 && vec_ok(p.q, p.sq, p.batch, p.heads, p.q_len, p.head_dim) &&
+                   vec_ok(p.k, p.sk, p.batch, p.kv_heads, p.kv_len, p.head_dim) &&
+                   vec_ok(p.v, p.sv, p.batch, p.kv_heads, p.kv_len, p.head_dim);
+  if (dtype == LSR_DTYPE_F32) return wide ? forward<float, 128>(p, vec, st) : forward<float, 64>(p, vec, st);
+  if (dtype == LSR_DTYPE_BF16) return wide ? forward<__nv_bfloat16, 128>(p, vec, st) : forward<__nv_bfloat16, 64>(p, vec, st);
+  return wide ? forward<__half, 128>(p, vec, st) : forward<__half, 64>(p, vec, st);
 }
 
 int attention_backward_general(const AttnParams& p, int dtype, cudaStream_t st) {
   const bool wide = p.head_dim > 64;
-  if (dtype == LSR_DTYPE_F32) return wide ? backward<float, 2>(p, st) : backward<float, 1>(p, st);
-  if (dtype == LSR_DTYPE_BF16) return wide ? backward<__nv_bfloat16, 2>(p, st) : backward<__nv_bfloat16, 1>(p, st);
-  return wide ? backward<__half, 2>(p, st) : backward<__half, 1>(p, st);
+  const bool vec = dtype == LSR_DTYPE_F32 && vec_ok(p.q, p.sq, p.batch, p.heads, p.q_len, p.head_dim) &&
+                   vec_ok(p.k, p.sk, p.batch, p.kv_heads, p.kv_len, p.head_dim) &&
+                   vec_ok(p.v, p.sv, p.batch, p.kv_heads, p.kv_len, p.head_dim) &&
+                   vec_ok(p.dout, p.sdo, p.batch, p.heads, p.q_len, p.head_dim);
+  if (dtype == LSR_DTYPE_F32) return wide ? backward<float, 128>(p, vec, st) : backward<float, 64>(p, vec, st);
+  if (dtype == LSR_DTYPE_BF16) return wide ? backward<__nv_bfloat16, 128>(p, vec, st) : backward<__nv_bfloat16, 64>(p, vec, st);
+  return wide ? backward<__half, 128>(p, vec, st) : backward<__half, 64>(p, vec, st);
 }
 
 }  // namespace lsr

@@ -105,8 +105,8 @@ def attention_forward(q, k, v, *, causal: bool = False, scale: float | None = No
     b, n, h, d = q.shape
     lib, dev = _lib.load(), q.device
     with _lib.on_device(dev):
-        out = torch.empty((b, n, h, d), dtype=q.dtype, device=dev)
-        lse = torch.empty((b, h, n), dtype=torch.float32, device=dev)
+        out = q.new_empty((b, n, h, d))
+        lse = q.new_empty((b, h, n), dtype=torch.float32)
         args = _pack(q, k, v, key_mask, causal, scale, out, lse)
         nbytes = lib.lsr_attention_forward_workspace_bytes(args)
         ws = _workspace(nbytes, dev)
@@ -125,10 +125,9 @@ def attention_backward(dout, q, k, v, out, lse, *, causal: bool = False, scale: 
         raise ValueError("lse must be fp32 [batch, heads, q_len] on q's device")
     dout, q, k, v, out, key_mask = _read(dout), _read(q), _read(k), _read(v), _read(out), _mask(key_mask)
     lse = lse.contiguous()
-    lib, dev, dtype = _lib.load(), q.device, q.dtype
+    lib, dev = _lib.load(), q.device
     with _lib.on_device(dev):
-        dq = torch.empty(q.shape, dtype=dtype, device=dev)
-        dk, dv = torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
         args = _pack(q, k, v, key_mask, causal, scale, out, lse, dout, dq, dk, dv)
         nbytes = lib.lsr_attention_backward_workspace_bytes(args)
         ws = _workspace(nbytes, dev)
