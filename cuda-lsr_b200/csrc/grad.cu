@@ -24,6 +24,8 @@ constexpr int GR_THREADS = 512;
 constexpr int GR_CHUNK = 1 << 15;  // entries
 constexpr int GR_TABLE = 1024;     // tensors per launch at most (30 bytes each of the 32764 bytes of kernel parameters)
 constexpr int GR_SMALL = 96;       // a shorter list takes kernels with 3 KB of parameters instead of 30: less to copy per launch
+constexpr int GR_CLUSTER = 8;      // blocks that take a short list in one launch
+constexpr int GR_SHORT = 64;       // chunks of a short list
 constexpr int GR_GRID = 592;       // blocks: 148 SMs x 4 blocks of 512 threads
 enum : int { NORM_MAX = 0, NORM_ONE = 1, NORM_TWO = 2 };
 
@@ -126,11 +128,11 @@ __device__ __forceinline__ void norm_chunk(const T* __restrict__ p, int n, Acc<K
   }
 }
 
+// The calling thread's part of the chunks first, first + step, ...
 template <int KIND, int N>
-__global__ void __launch_bounds__(GR_THREADS) grad_norm_kernel(const __grid_constant__ GradTable<N> t,
-                                                               Acc<KIND>* __restrict__ partial) {
+__device__ __forceinline__ Acc<KIND> norm_chunks(const GradTable<N>& t, int first, int step) {
   Acc<KIND> acc;
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+  for (int c = first; c < t.chunks; c += step) {
     const int k = find_tensor(t, c);
     const long long at = (long long)(c - t.first[k]) * GR_CHUNK;
     const int n = (int)min((long long)GR_CHUNK, t.numel[k] - at);
@@ -138,7 +140,13 @@ __global__ void __launch_bounds__(GR_THREADS) grad_norm_kernel(const __grid_cons
     else if (t.tin[k] == LSR_DTYPE_BF16) norm_chunk(static_cast<const __nv_bfloat16*>(t.in[k]) + at, n, acc);
     else norm_chunk(static_cast<const __half*>(t.in[k]) + at, n, acc);
   }
-  acc = block_sum(acc);
+  return acc;
+}
+
+template <int KIND, int N>
+__global__ void __launch_bounds__(GR_THREADS) grad_norm_kernel(const __grid_constant__ GradTable<N> t,
+                                                               Acc<KIND>* __restrict__ partial) {
+  const Acc<KIND> acc = block_sum(norm_chunks<KIND>(t, (int)blockIdx.x, (int)gridDim.x));
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
@@ -192,19 +200,15 @@ __device__ __forceinline__ void scale_chunk_to(const TI* p, void* out, int tout,
   else scale_chunk(p, static_cast<__half*>(out) + at, n, coef);
 }
 
-// GIVEN: *norm is read (a norm of more tensors than these); else it is the partials' and is written.
-template <int KIND, bool GIVEN, int N>
-__global__ void __launch_bounds__(GR_THREADS) grad_scale_kernel(const __grid_constant__ GradTable<N> t,
-                                                                const Acc<KIND>* __restrict__ partial, int npartial,
-                                                                float max_norm, float* norm, int write_norm) {
-  float total;
-  if (GIVEN) total = *norm;
-  else total = total_norm<KIND>(partial, npartial);
-  if (!GIVEN && write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
-  float coef = max_norm / (total + 1e-6f);
-  coef = coef > 1.f ? 1.f : coef;  // a NaN stays
-  // the last chunks first: those are the ones that the pass before left in L2
-  for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= (int)gridDim.x) {
+__device__ __forceinline__ float coefficient(float total, float max_norm) {
+  const float c = max_norm / (total + 1e-6f);
+  return c > 1.f ? 1.f : c;  // a NaN stays
+}
+
+// The last chunks first: those are the ones that the pass before left in L2.
+template <int N>
+__device__ __forceinline__ void scale_chunks(const GradTable<N>& t, float coef, int first, int step) {
+  for (int c = t.chunks - 1 - first; c >= 0; c -= step) {
     const int k = find_tensor(t, c);
     if (coef == 1.f && t.in[k] == t.out[k]) continue;  // nothing changes
     const long long at = (long long)(c - t.first[k]) * GR_CHUNK;
@@ -214,6 +218,42 @@ __global__ void __launch_bounds__(GR_THREADS) grad_scale_kernel(const __grid_con
       scale_chunk_to(static_cast<const __nv_bfloat16*>(t.in[k]) + at, t.out[k], t.tout[k], at, n, coef);
     else scale_chunk_to(static_cast<const __half*>(t.in[k]) + at, t.out[k], t.tout[k], at, n, coef);
   }
+}
+
+// A short list in one launch: the blocks of one cluster take the chunks, read one another's sums from shared
+// memory, add them in rank order, and (CLIP) scale what they have just read.
+template <int KIND, bool CLIP, int N>
+__global__ void __cluster_dims__(GR_CLUSTER) __launch_bounds__(GR_THREADS)
+    grad_short_kernel(const __grid_constant__ GradTable<N> t, float max_norm, float* __restrict__ norm) {
+  __shared__ Acc<KIND> sum;
+  const int rank = (int)cluster_ctarank();
+  const Acc<KIND> own = block_sum(norm_chunks<KIND>(t, rank, GR_CLUSTER));
+  if (threadIdx.x == 0) sum = own;
+  cluster_sync_all();
+  Acc<KIND> all;
+#pragma unroll
+  for (int r = 0; r < GR_CLUSTER; ++r) {
+    Acc<KIND> other;
+    asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(*reinterpret_cast<unsigned long long*>(&other.s))
+                 : "r"(mapa_shared(smem_u32(&sum), r)) : "memory");
+    all.join(other);
+  }
+  cluster_sync_all();  // nobody leaves while its sum may be read
+  const float total = all.norm();
+  if (rank == 0 && threadIdx.x == 0) *norm = total;
+  if (CLIP) scale_chunks(t, coefficient(total, max_norm), rank, GR_CLUSTER);
+}
+
+// GIVEN: *norm is read (a norm of more tensors than these); else it is the partials' and is written.
+template <int KIND, bool GIVEN, int N>
+__global__ void __launch_bounds__(GR_THREADS) grad_scale_kernel(const __grid_constant__ GradTable<N> t,
+                                                                const Acc<KIND>* __restrict__ partial, int npartial,
+                                                                float max_norm, float* norm, int write_norm) {
+  float total;
+  if (GIVEN) total = *norm;
+  else total = total_norm<KIND>(partial, npartial);
+  if (!GIVEN && write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
+  scale_chunks(t, coefficient(total, max_norm), (int)blockIdx.x, (int)gridDim.x);
 }
 
 bool dtype_ok(int d) { return d == LSR_DTYPE_F32 || d == LSR_DTYPE_BF16 || d == LSR_DTYPE_F16; }
@@ -320,6 +360,13 @@ template <int KIND, int N>
 int norm_table(const void* const* in, const long long* numel, const int* tin, int n, float* norm, void* ws, size_t bytes,
               cudaStream_t st) {
   GradTable<N> t;
+  int taken = 0;
+  fill_table(t, in, nullptr, numel, tin, nullptr, n, &taken);
+  if (taken == n && t.chunks <= GR_SHORT) {
+    ProfScope prof(PK_EW_OTHER, st);
+    grad_short_kernel<KIND, false, N><<<GR_CLUSTER, GR_THREADS, 0, st>>>(t, 0.f, norm);
+    return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
+  }
   auto* partial = static_cast<Acc<KIND>*>(ws);
   int count = 0;
   const int rc = launch_partials<KIND, N>(t, in, numel, tin, n, partial, (int)(bytes / sizeof(double)), &count, st);
@@ -336,6 +383,13 @@ int clip_table(const void* const* in, void* const* out, const long long* numel, 
   auto* partial = static_cast<Acc<KIND>*>(ws);
   int count = 0;
   if (!GIVEN) {
+    int taken = 0;
+    fill_table(t, in, out, numel, tin, tout, n, &taken);
+    if (taken == n && t.chunks <= GR_SHORT) {
+      ProfScope prof(PK_EW_OTHER, st);
+      grad_short_kernel<KIND, true, N><<<GR_CLUSTER, GR_THREADS, 0, st>>>(t, max_norm, norm);
+      return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
+    }
     const int rc = launch_partials<KIND, N>(t, in, numel, tin, n, partial, (int)(bytes / sizeof(double)), &count, st);
     if (rc != LSR_OK) return rc;
   }

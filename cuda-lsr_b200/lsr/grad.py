@@ -31,12 +31,7 @@ _KINDS = {math.inf: 0, 1.0: 1, 2.0: 2}
 # A model has hundreds of gradients: their properties are read by map over the unbound getters.
 _ptr_of, _numel_of, _size_of, _is_contiguous = (torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.size,
                                                 torch.Tensor.is_contiguous)
-_layout_of, _device_of, _dtype_of = (torch.Tensor.layout.__get__, torch.Tensor.device.__get__,
-                                     torch.Tensor.dtype.__get__)
-
-
-def _is_tensor(t) -> bool:
-    return isinstance(t, torch.Tensor)
+_device_of, _dtype_of = torch.Tensor.get_device, torch.Tensor.dtype.__get__
 
 
 def _kind(norm_type) -> int:
@@ -58,29 +53,31 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _check_list(tensors, what: str) -> list[torch.Tensor]:
+def _check_list(tensors, what: str):
+    """(tensors, their addresses, element types, whether every one is contiguous)"""
     ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not all(map(_is_tensor, ts)):
-        raise ValueError(f"{what} must be tensors")
-    layouts, devices, dtypes = set(map(_layout_of, ts)), set(map(_device_of, ts)), set(map(_dtype_of, ts))
-    if layouts - {torch.strided}:
-        raise ValueError(f"{what} must be dense tensors (got {layouts - {torch.strided}})")
-    if any(d.type != "cuda" for d in devices):
+    try:
+        dtypes, devices = list(map(_dtype_of, ts)), set(map(_device_of, ts))
+        ptrs, whole = array("Q", map(_ptr_of, ts)), all(map(_is_contiguous, ts))
+    except (TypeError, RuntimeError, NotImplementedError):  # no tensor, or one without plain memory (sparse, meta)
+        raise ValueError(f"{what} must be dense tensors") from None
+    if -1 in devices:
         raise ValueError(f"{what} must be CUDA tensors (liblsr has no CPU path)")
-    if dtypes - _lib.DTYPE_CODES.keys():
-        raise ValueError(f"{what} must be fp32, bf16 or fp16 (got {dtypes - _lib.DTYPE_CODES.keys()})")
     if len(devices) > 1:
-        raise ValueError(f"{what} must be on one device (got {devices})")
-    return ts
+        raise ValueError(f"{what} must be on one device (got CUDA devices {sorted(devices)})")
+    kinds = set(dtypes)
+    if kinds - _lib.DTYPE_CODES.keys():
+        raise ValueError(f"{what} must be fp32, bf16 or fp16 (got {kinds - _lib.DTYPE_CODES.keys()})")
+    if len(kinds) == 1:
+        codes = array("i", (_lib.DTYPE_CODES[dtypes[0]],)) * len(ts)
+    else:
+        codes = array("i", [_lib.DTYPE_CODES[t] for t in dtypes])
+    return ts, ptrs, codes, whole
 
 
-def _arrays(ts):
-    return array("Q", list(map(_ptr_of, ts))), array("i", [_lib.DTYPE_CODES[t] for t in map(_dtype_of, ts)])
-
-
-def _workspace(lib, count: int, device: torch.device) -> torch.Tensor:
+def _workspace(lib, count: int, like: torch.Tensor) -> torch.Tensor:
     # of this call alone: calls on several streams, or graphs captured here, share nothing
-    return torch.empty(lib.lsr_grad_workspace_bytes(count), dtype=torch.uint8, device=device)
+    return like.new_empty(lib.lsr_grad_workspace_bytes(count), dtype=torch.uint8)
 
 
 def _address(a: array) -> int:
@@ -97,7 +94,7 @@ def _flatten(ts, outs):
             continue
         if any(st == 0 and sz > 1 for st, sz in zip(o.stride(), o.shape)):
             raise ValueError("an output's entries share memory (an expanded tensor): clip a copy of it")
-        src.append(t.contiguous())
+        src.append(t.detach().contiguous())
         if o.is_contiguous():
             dst.append(o)
         else:
@@ -106,24 +103,23 @@ def _flatten(ts, outs):
     return src, dst, back
 
 
-@torch.no_grad()
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """The norm (1, 2 or inf) over every entry of every tensor: a 0-d fp32 tensor on their device."""
     kind = _kind(norm_type)
-    ts = _check_list(tensors, "tensors")
+    ts, ptrs, dtypes, whole = _check_list(tensors, "tensors")
     if not ts:
         return torch.zeros(())
-    if not all(map(_is_contiguous, ts)):
-        ts = [t if _dense(t) else t.contiguous() for t in ts]
-    dev = ts[0].device
+    if not whole:
+        ts = [t if _dense(t) else t.detach().contiguous() for t in ts]
+        ptrs = array("Q", map(_ptr_of, ts))
+    first = ts[0]
     lib = _lib.load()
-    with _lib.on_device(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws = _workspace(lib, len(ts), dev)
-        ptrs, dtypes = _arrays(ts)
-        numel = array("q", list(map(_numel_of, ts)))
+    with _lib.on_device(first.device):
+        norm = first.new_empty((), dtype=torch.float32)
+        ws = _workspace(lib, len(ts), first)
+        numel = array("q", map(_numel_of, ts))
         rc = lib.lsr_grad_norm(_address(ptrs), _address(numel), _address(dtypes), len(ts), kind, norm.data_ptr(),
-                               ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
+                               ws.data_ptr(), ws.numel(), _lib.stream_handle(first.device))
     _lib.check(rc, "lsr_grad_norm")
     return norm
 
@@ -142,27 +138,30 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be at least 0 (got {max_norm})")
-    ts = _check_list(grads, "grads")
-    outs = ts if out is None else _check_list(out, "out")
-    if outs is not ts and list(map(_size_of, outs)) != list(map(_size_of, ts)):
-        raise ValueError("out must be one tensor of the same shape for each gradient")
-    if not ts:
+    src, pin, tin, whole = _check_list(grads, "grads")
+    dst, pout, tout = src, pin, tin
+    if out is not None:
+        dst, pout, tout, same = _check_list(out, "out")
+        whole = whole and same
+        if list(map(_size_of, dst)) != list(map(_size_of, src)):
+            raise ValueError("out must be one tensor of the same shape for each gradient")
+    if not src:
         return torch.zeros(()) if total_norm is None else total_norm
-    dev = ts[0].device
-    if outs[0].device != dev:
+    first = src[0]
+    dev = first.device
+    if dst[0].get_device() != first.get_device():
         raise ValueError("out must be on the gradients' device")
     if total_norm is not None and (total_norm.dtype != torch.float32 or total_norm.device != dev or total_norm.numel() != 1):
         raise ValueError("total_norm must be one fp32 value on the gradients' device")
-    src, dst, back = ts, outs, []
-    if not (all(map(_is_contiguous, ts)) and (outs is ts or all(map(_is_contiguous, outs)))):
-        src, dst, back = _flatten(ts, outs)
+    back = []  # (output, dense tensor to copy into it)
+    if not whole:
+        src, dst, back = _flatten(src, dst)
+        pin, pout = array("Q", map(_ptr_of, src)), array("Q", map(_ptr_of, dst))
     lib = _lib.load()
     with _lib.on_device(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev) if total_norm is None else total_norm
-        ws = _workspace(lib, len(src), dev) if total_norm is None else None
-        pin, tin = _arrays(src)
-        pout, tout = _arrays(dst)
-        numel = array("q", list(map(_numel_of, src)))
+        norm = first.new_empty((), dtype=torch.float32) if total_norm is None else total_norm
+        ws = _workspace(lib, len(src), first) if total_norm is None else None
+        numel = array("q", map(_numel_of, src))
         rc = lib.lsr_grad_clip(_address(pin), _address(pout), _address(numel), _address(tin), _address(tout), len(src),
                                kind, max_norm, int(total_norm is not None), norm.data_ptr(),
                                ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
@@ -173,7 +172,6 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
     return norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """Clip the gradients of `parameters` in place by their global norm and return it (0-d fp32).
 
