@@ -42,6 +42,9 @@ struct BwdParams {
   float* stats;  // [batch][heads][query tiles][2][128]: lse log2 e - extra (plus infinity: no probability), D 2^-extra
   int q_tiles, kv_tiles;
   long long kv_blocks;
+  // blocks that the steps of 128 keys, and of 128 queries, are dealt to; with more than one their sums go here
+  int split_k, split_q;
+  float *part_dk, *part_dv, *part_dq;  // [split][batch][head][position][dim]
 };
 
 template <int PANELS, bool MASK>
@@ -57,6 +60,7 @@ struct BwdSmem {
 // Row statistics, eight lanes per row.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ BwdParams p) {
+  launch_dependents();
   const long long row = (long long)blockIdx.x * 32 + threadIdx.x / 8;  // rows of whole tiles
   const int len = p.q_tiles * kRows, part = threadIdx.x % 8;
   const int i = (int)(row % len), h = (int)(row / len % p.a.heads), b = (int)(row / len / p.a.heads);
@@ -112,6 +116,20 @@ __device__ __forceinline__ void store_rows(T* dst, uint32_t at, int col0, int co
   }
 }
 
+// The same in 32 bits, as it is.
+__device__ __forceinline__ void store_part(float* dst, uint32_t at, int col0, int col1, int dim, bool live, bool any) {
+  for (int q = col0; q < col1; q += 32) {
+    uint32_t o[32];
+    tmem_ld32(at + q, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; e += 4)
+      if (live && q + e < dim)
+        *reinterpret_cast<uint4*>(dst + q + e) =
+            any ? make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_uint4(0, 0, 0, 0);
+  }
+}
+
 template <typename T, int PANELS, bool MASK, bool KEYS>
 __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_t* smem) {
   using L = BwdSmem<PANELS, MASK>;
@@ -128,6 +146,12 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
   int* status = p.a.status;
 
   // the block's rows, and the tiles of the other side that it passes over
+  const int splits = KEYS ? p.split_k : p.split_q;
+  int split = 0;
+  if (splits > 1) {
+    split = (int)(x % splits);
+    x /= splits;
+  }
   int tile, h, b, first = 0, tiles;
   if (KEYS) {
     tile = (int)(x % p.kv_tiles);  // under causality the first keys are seen by the most queries
@@ -147,7 +171,7 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
   const int row0 = tile * kRows;
   const unsigned char* mask = MASK ? p.a.mask + b * p.a.mask_stride : nullptr;
 
-  if (threadIdx.x == 0) {
+  if (warp == LOADER && lane == 0) {
     mbar_init(fixed, 1);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full + s, 1);
@@ -160,6 +184,38 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
+  }
+  // steps: query tiles of every head of the group, or tiles of keys of which some are seen
+  int steps = KEYS ? tiles * p.a.group : tiles, begin = 0;
+  if (splits > 1) {  // this block's share of them
+    const int share = (steps + splits - 1) / splits;
+    begin = min(steps, split * share);
+    steps = min(steps, begin + share);
+  }
+  auto load_fixed = [&] {
+    mbar_arrive_expect_tx(fixed, 2 * L::TILE);
+#pragma unroll
+    for (int i = 0; i < PANELS; ++i) {
+      tma_load_4d(r1 + i * kPanel, KEYS ? &p.mk : &p.mq, fixed, i * 64, row0, h, b);
+      tma_load_4d(r2 + i * kPanel, KEYS ? &p.mv : &p.mdo, fixed, i * 64, row0, h, b);
+    }
+  };
+  // operand k (0: queries with their statistics, or keys; 1: dout, or values) of step j, into a stage
+  auto load_step = [&](int j, int k, int s) {
+    const int t = KEYS ? first + j % tiles : j, hh = KEYS ? h * p.a.group + j / tiles : h / p.a.group;
+    const bool stats = KEYS && k == 0;
+    mbar_arrive_expect_tx(full + s, L::TILE + (stats ? 1024 : 0));
+    const CUtensorMap* map = KEYS ? (k ? &p.mdo : &p.mq) : (k ? &p.mv : &p.mk);
+#pragma unroll
+    for (int i = 0; i < PANELS; ++i) tma_load_4d(ring + s * L::TILE + i * kPanel, map, full + s, i * 64, t * kRows, hh, b);
+    if (stats)
+      bulk_load(smem + L::STATS + s / 2 * 1024, p.stats + (((long long)b * p.a.heads + hh) * p.q_tiles + t) * 256, 1024,
+                full + s);
+  };
+  // Without a mask the first loads go out before the block is set up; the statistics are the kernel's before.
+  if (!MASK && warp == LOADER && lane == 0 && begin < steps) {
+    load_fixed();
+    if (!KEYS) load_step(begin, 0, 0), load_step(begin, 1, 1);
   }
   if (MASK && !KEYS)
     pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS), mask, tiles, p.a.kv_len, warp, BWD_THREADS / 32, lane);
@@ -175,43 +231,28 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
   tc_fence_before();
   // a tile of masked keys alone has nothing to do
   if (MASK && KEYS) {
-    if (!__syncthreads_or(!dead_key && row0 + (int)threadIdx.x % kRows < p.a.kv_len)) tiles = 0;
+    if (!__syncthreads_or(!dead_key && row0 + (int)threadIdx.x % kRows < p.a.kv_len)) steps = begin;
   } else {
     __syncthreads();
   }
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, t1 = tmem, t2 = tmem + 128, acc1 = tmem + 256, acc2 = tmem + 256 + 64 * PANELS;
   const KeyBits bits{MASK && !KEYS ? reinterpret_cast<const uint4*>(smem + L::BITS) : nullptr};
-  // steps: query tiles of every head of the group, or tiles of keys of which some are seen
-  const int steps = KEYS ? tiles * p.a.group : tiles;
-  const int start = bits.next(0, steps);
+  const int start = bits.next(begin, steps);
 
   if (warp >= LOADER) {
     regs_dec<kRestRegs>();
     if (warp == LOADER) {
       if (lane == 0 && start < steps) {
-        mbar_arrive_expect_tx(fixed, 2 * L::TILE);
-#pragma unroll
-        for (int i = 0; i < PANELS; ++i) {
-          tma_load_4d(r1 + i * kPanel, KEYS ? &p.mk : &p.mq, fixed, i * 64, row0, h, b);
-          tma_load_4d(r2 + i * kPanel, KEYS ? &p.mv : &p.mdo, fixed, i * 64, row0, h, b);
-        }
+        if (MASK) load_fixed();
+        if (KEYS) wait_dependency();
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
         for (int j = start; ok && j < steps; j = bits.next(j + 1, steps)) {
-          const int t = KEYS ? first + j % tiles : j, hh = KEYS ? h * p.a.group + j / tiles : h / p.a.group;
           for (int k = 0; k < 2; ++k) {
             if (!(ok = mbar_wait(empty + s, ph ^ 1, abort_flag, status, ST_ATTN_LOAD))) break;
-            uint8_t* dst = ring + s * L::TILE;
-            const bool stats = KEYS && k == 0;
-            mbar_arrive_expect_tx(full + s, L::TILE + (stats ? 1024 : 0));
-            const CUtensorMap* map = KEYS ? (k ? &p.mdo : &p.mq) : (k ? &p.mv : &p.mk);
-#pragma unroll
-            for (int i = 0; i < PANELS; ++i) tma_load_4d(dst + i * kPanel, map, full + s, i * 64, t * kRows, hh, b);
-            if (stats)
-              bulk_load(smem + L::STATS + s / 2 * 1024, p.stats + (((long long)b * p.a.heads + hh) * p.q_tiles + t) * 256, 1024,
-                        full + s);
+            if (MASK || KEYS || j > start) load_step(j, k, s);
             if (++s == STAGES) s = 0, ph ^= 1;
           }
         }
@@ -302,6 +343,7 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
     uint32_t sph = 0;
     float lse = 0.f, delta = 0.f;
     if (!KEYS) {
+      wait_dependency();
       const float* st = p.stats + (((long long)b * p.a.heads + h) * p.q_tiles + tile) * 256 + r;
       lse = st[0] + (float)kExtra<T>;
       delta = st[128] * (float)(1 << kExtra<T>);
@@ -396,10 +438,17 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
     tc_fence_after();
     if (ok) {
       const bool any = start < steps && !dead_key;
-      if (KEYS) {  // half of the warpgroups store dv, half dk, each its share of the columns
-        constexpr int SHARE = 64 * PANELS / (PARTS / 2);
-        const bool live = row < p.a.kv_len, second = part >= PARTS / 2;
-        const int col = part % (PARTS / 2) * SHARE;
+      constexpr int SHARE = 64 * PANELS / (PARTS / 2);  // half of the warpgroups store dv, half dk
+      const bool second = part >= PARTS / 2;
+      const int col = part % (PARTS / 2) * SHARE;
+      if (splits > 1) {
+        const int len = KEYS ? p.a.kv_len : p.a.q_len, heads = KEYS ? p.a.kv_heads : p.a.heads;
+        float* to = (KEYS ? (second ? p.part_dk : p.part_dv) : p.part_dq) +
+                    ((((long long)split * p.a.batch + b) * heads + h) * len + row) * p.a.head_dim;
+        if (KEYS) store_part(to, (second ? acc2 : acc1) + quarter, col, col + SHARE, p.a.head_dim, row < len, any);
+        else if (part < 2 * PANELS) store_part(to, acc2 + quarter, part * 32, part * 32 + 32, p.a.head_dim, row < len, any);
+      } else if (KEYS) {
+        const bool live = row < p.a.kv_len;
         if (!second)
           store_rows(attn_at<T>(p.a.dv, p.a.sdv, b, h) + row * p.a.sdv.s, acc1 + quarter, col, col + SHARE, p.a.head_dim, live, any,
                      1.f / (1 << kExtra<T>));
@@ -428,12 +477,41 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) attn_bwd_kernel(const __grid_c
   else bwd_block<T, PANELS, MASK, false>(p, blockIdx.x - (unsigned)p.kv_blocks, smem);
 }
 
+// The sums of several blocks added in order and rounded, a warp per row of dq, dk or dv.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_grads_kernel(const __grid_constant__ BwdParams p) {
+  const long long rq = p.split_q > 1 ? (long long)p.a.batch * p.a.heads * p.a.q_len : 0;
+  const long long rk = p.split_k > 1 ? (long long)p.a.batch * p.a.kv_heads * p.a.kv_len : 0;
+  long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
+  if (row >= rq + 2 * rk) return;
+  const int which = row < rq ? 0 : row < rq + rk ? 1 : 2;  // dq, dk, dv
+  row -= which == 0 ? 0 : which == 1 ? rq : rq + rk;
+  const int len = which ? p.a.kv_len : p.a.q_len, heads = which ? p.a.kv_heads : p.a.heads;
+  const int splits = which ? p.split_k : p.split_q, e = threadIdx.x % 32 * 4;
+  if (e >= p.a.head_dim) return;
+  const float* from = (which == 0 ? p.part_dq : which == 1 ? p.part_dk : p.part_dv) + row * p.a.head_dim + e;
+  const long long step = (which ? rk : rq) * p.a.head_dim;
+  float x[4] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(from + s * step);
+    x[0] += v.x;
+    x[1] += v.y;
+    x[2] += v.z;
+    x[3] += v.w;
+  }
+  const float mul = which == 2 ? 1.f / (1 << kExtra<T>) : p.a.scale;
+  const int i = (int)(row % len), h = (int)(row / len % heads), b = (int)(row / len / heads);
+  const AttnStride& sd = which == 0 ? p.a.sdq : which == 1 ? p.a.sdk : p.a.sdv;
+  T* dst = attn_at<T>(which == 0 ? p.a.dq : which == 1 ? p.a.dk : p.a.dv, sd, b, h) + i * sd.s + e;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(x[0] * mul, x[1] * mul), pack2<T>(x[2] * mul, x[3] * mul));
+}
+
 template <typename T, int PANELS, bool MASK>
 int launch(BwdParams& p, cudaStream_t st) {
   using L = BwdSmem<PANELS, MASK>;
   static_assert(L::TOTAL <= 232448, "shared memory budget exceeded");
   const long long rows = (long long)p.q_tiles * kRows * p.a.heads * p.a.batch;
-  const long long blocks = p.kv_blocks + (long long)p.q_tiles * p.a.heads * p.a.batch;
+  const long long blocks = p.kv_blocks + (long long)p.q_tiles * p.a.heads * p.a.batch * p.split_q;
   if (blocks > 0x7fffffffll || rows / 32 > 0x7fffffffll) return LSR_ERR_SHAPE;
   {
     ProfScope prof(PK_EW_OTHER, st);
@@ -443,9 +521,43 @@ int launch(BwdParams& p, cudaStream_t st) {
   auto kernel = attn_bwd_kernel<T, PANELS, MASK>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess)
     return LSR_ERR_LAUNCH;
-  ProfScope prof(PK_GEMM_OTHER, st);
-  kernel<<<(unsigned)blocks, BWD_THREADS, L::TOTAL, st>>>(p);
+  {
+    ProfScope prof(PK_GEMM_OTHER, st);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(BWD_THREADS);
+    cfg.dynamicSmemBytes = L::TOTAL;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the blocks are set up while the statistics are taken
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return LSR_ERR_LAUNCH;
+  }
+  const long long joined = (p.split_q > 1 ? (long long)p.a.batch * p.a.heads * p.a.q_len : 0) +
+                           (p.split_k > 1 ? 2ll * p.a.batch * p.a.kv_heads * p.a.kv_len : 0);
+  if (joined == 0) return LSR_OK;
+  ProfScope prof(PK_EW_OTHER, st);
+  attn_join_grads_kernel<T><<<(unsigned)((joined + 7) / 8), 256, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
+}
+
+// Blocks that the steps of one set of rows are dealt to: one, unless they are one and a half times what an SM
+// has on average or more (few keys under many queries, or few queries over many keys), and four steps at least.
+int split_count(long long steps, long long mean) {
+  mean = std::max<long long>(mean, 4);
+  return 2 * steps >= 3 * mean ? (int)std::min<long long>((steps + mean - 1) / mean, 64) : 1;
+}
+
+void set_splits(BwdParams& p) {
+  p.q_tiles = cdiv(p.a.q_len, kRows);
+  p.kv_tiles = cdiv(p.a.kv_len, kRows);
+  const long long k_sets = (long long)p.kv_tiles * p.a.kv_heads * p.a.batch, k_steps = (long long)p.q_tiles * p.a.group;
+  const long long q_sets = (long long)p.q_tiles * p.a.heads * p.a.batch, q_steps = p.kv_tiles;
+  const long long sms = device_sm_count(), mean = (k_sets * k_steps + q_sets * q_steps + sms - 1) / sms;
+  p.split_k = split_count(k_steps, mean);
+  p.split_q = split_count(q_steps, mean);
 }
 
 template <typename T>
@@ -456,17 +568,26 @@ int backward(BwdParams& p, cudaStream_t st) {
 
 }  // namespace
 
-size_t attention_backward_sm100_ws(const AttnParams& p) {
-  return (size_t)cdiv(p.q_len, kRows) * p.heads * p.batch * 256 * sizeof(float);
+size_t attention_backward_sm100_ws(const AttnParams& a) {
+  BwdParams p{};
+  p.a = a;
+  set_splits(p);
+  size_t floats = (size_t)p.q_tiles * a.heads * a.batch * 256;
+  if (p.split_k > 1) floats += (size_t)p.split_k * 2 * a.batch * a.kv_heads * a.kv_len * a.head_dim;
+  if (p.split_q > 1) floats += (size_t)p.split_q * a.batch * a.heads * a.q_len * a.head_dim;
+  return floats * sizeof(float);
 }
 
 int attention_backward_sm100(const AttnParams& a, int dtype, void* ws, cudaStream_t st) {
   BwdParams p{};
   p.a = a;
+  set_splits(p);
   p.stats = static_cast<float*>(ws);
-  p.q_tiles = cdiv(a.q_len, kRows);
-  p.kv_tiles = cdiv(a.kv_len, kRows);
-  p.kv_blocks = (long long)p.kv_tiles * a.kv_heads * a.batch;
+  p.part_dk = p.stats + (size_t)p.q_tiles * a.heads * a.batch * 256;
+  const size_t kv = p.split_k > 1 ? (size_t)p.split_k * a.batch * a.kv_heads * a.kv_len * a.head_dim : 0;
+  p.part_dv = p.part_dk + kv;
+  p.part_dq = p.part_dv + kv;
+  p.kv_blocks = (long long)p.kv_tiles * a.kv_heads * a.batch * p.split_k;
   int rc = encode_rows(&p.mq, a.q, a.sq, a.batch, a.heads, a.q_len, a.head_dim, dtype);
   if (rc == LSR_OK) rc = encode_rows(&p.mdo, a.dout, a.sdo, a.batch, a.heads, a.q_len, a.head_dim, dtype);
   if (rc == LSR_OK) rc = encode_rows(&p.mk, a.k, a.sk, a.batch, a.kv_heads, a.kv_len, a.head_dim, dtype);

@@ -168,6 +168,16 @@ def test_rows_before_the_first_key_are_empty(dtype):
     assert bool((c.grads[0][:, :260] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("n,m,h,hk,d,causal,masked", [(5, 1500, 2, 1, 64, True, False), (1500, 60, 4, 1, 64, False, False),
+                                                      (3, 2000, 1, 1, 128, True, True), (1100, 130, 2, 2, 80, False, True)])
+def test_few_rows_whose_steps_are_dealt_to_several_blocks(n, m, h, hk, d, causal, masked, dtype):
+    mask = torch.arange(m, device="cuda")[None] % 7 != 3 if masked else None
+    if masked and m > 1000:
+        mask = mask & (torch.arange(m, device="cuda")[None] > 700)  # the first blocks' keys are all hidden
+    Case(*tensors(1, n, m, h, hk, d, dtype, seed=n), causal=causal, key_mask=mask)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("spread", [0.0, 30.0])
 def test_flat_and_peaked_rows(dtype, spread):
