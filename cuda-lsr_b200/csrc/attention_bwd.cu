@@ -212,11 +212,6 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
       bulk_load(smem + L::STATS + s / 2 * 1024, p.stats + (((long long)b * p.a.heads + hh) * p.q_tiles + t) * 256, 1024,
                 full + s);
   };
-  // Without a mask the first loads go out before the block is set up; the statistics are the kernel's before.
-  if (!MASK && warp == LOADER && lane == 0 && begin < steps) {
-    load_fixed();
-    if (!KEYS) load_step(begin, 0, 0), load_step(begin, 1, 1);
-  }
   if (MASK && !KEYS)
     pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS), mask, tiles, p.a.kv_len, warp, BWD_THREADS / 32, lane);
   if (warp == ISSUER) {
@@ -244,7 +239,7 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
     regs_dec<kRestRegs>();
     if (warp == LOADER) {
       if (lane == 0 && start < steps) {
-        if (MASK) load_fixed();
+        load_fixed();
         if (KEYS) wait_dependency();
         int s = 0;
         uint32_t ph = 0;
@@ -252,10 +247,12 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
         for (int j = start; ok && j < steps; j = bits.next(j + 1, steps)) {
           for (int k = 0; k < 2; ++k) {
             if (!(ok = mbar_wait(empty + s, ph ^ 1, abort_flag, status, ST_ATTN_LOAD))) break;
-            if (MASK || KEYS || j > start) load_step(j, k, s);
+            load_step(j, k, s);
             if (++s == STAGES) s = 0, ph ^= 1;
           }
         }
+        drain_loads<STAGES>(full, s, ph, status);
+        drain_loads<1>(fixed, 1, 0, status);
       }
       __syncwarp();
     } else if (warp == ISSUER) {

@@ -113,12 +113,6 @@ __global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1) attn_fwd_kern
     mbar_init(done, ISSUERS);
     *abort_flag = 0;
     fence_mbar_init();
-    if (!MASK && first < most) {  // without a mask the first loads go out before the block is set up
-      for (int w = 0; w < NQ; ++w)
-        if (n[w] > first) load_rows<PANELS>(sq + w * L::TILE, &p.mq, q_full + w, i0 + w * kRows, h, b);
-      load_rows<PANELS>(skv, &p.mk, full, first * kRows, hk, b);
-      load_rows<PANELS>(skv + L::TILE, &p.mv, full + 1, first * kRows, hk, b);
-    }
   }
   if (MASK)
     pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS), p.a.mask + b * p.a.mask_stride, most, p.a.kv_len, warp,
@@ -145,16 +139,18 @@ __global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1) attn_fwd_kern
         uint32_t ph = 0;
         bool ok = true;
         const int j0 = bits.next(first, most);
-        if (MASK)
-          for (int w = 0; w < NQ; ++w)
-            if (n[w] > j0) load_rows<PANELS>(sq + w * L::TILE, &p.mq, q_full + w, i0 + w * kRows, h, b);
+        for (int w = 0; w < NQ; ++w)
+          if (n[w] > j0) load_rows<PANELS>(sq + w * L::TILE, &p.mq, q_full + w, i0 + w * kRows, h, b);
         for (int j = j0; ok && j < most; j = bits.next(j + 1, most)) {
           for (int kv = 0; kv < 2; ++kv) {
             if (!(ok = mbar_wait(empty + s, ph ^ 1, abort_flag, p.a.status, ST_ATTN_LOAD))) break;
-            if (MASK || j > j0) load_rows<PANELS>(skv + s * L::TILE, kv ? &p.mv : &p.mk, full + s, j * kRows, hk, b);
+            load_rows<PANELS>(skv + s * L::TILE, kv ? &p.mv : &p.mk, full + s, j * kRows, hk, b);
             if (++s == STAGES) s = 0, ph ^= 1;
           }
         }
+        drain_loads<STAGES>(full, s, ph, p.a.status);
+        for (int w = 0; w < NQ; ++w)
+          if (n[w] > j0) drain_loads<1>(q_full + w, 1, 0, p.a.status);
       }
       __syncwarp();
     } else if (warp < ISSUER + ISSUERS) {

@@ -93,6 +93,19 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, ok);
 }
 
+// Before a block ends, also after a wait that ran out: its copies into shared memory have landed (`bars` count
+// them, a ring of N; the next copy would have gone to stage s in phase ph). Bounded like every wait.
+template <int N>
+__device__ __forceinline__ void drain_loads(uint64_t* bars, int s, uint32_t ph, int* status) {
+  const uint64_t t0 = globaltimer_ns();
+  for (int i = 0; i < N; ++i)
+    while (!mbar_try_wait(bars + i, i < s ? ph : ph ^ 1))
+      if (globaltimer_ns() - t0 > LSR_WAIT_TIMEOUT_NS) {
+        set_status(status, ST_ATTN_DONE);
+        return;
+      }
+}
+
 // One arrival for a whole warp, after what its lanes did before (moves to and from TMEM included).
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   tc_fence_before();
