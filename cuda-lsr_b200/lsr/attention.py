@@ -9,9 +9,10 @@ q is [batch, q_len, heads, dim], k and v [batch, kv_len, kv_heads, dim], heads a
 strides: the three parts of one projection's output or [batch, heads, length, dim] tensors transposed are
 read in place; what is expanded, not on 16-byte boundaries or not contiguous within a head is copied first.
 ``causal`` lets query i see keys up to i + kv_len - q_len, so that the last query sees the last key.
-``key_mask`` is bool [batch, kv_len], True = seen; what the masked keys hold does not matter. A query
-that sees no key has output 0, lse minus infinity and no gradient. lse is fp32 [batch, heads, q_len],
-the natural logarithm. ``scale`` defaults to dim ** -0.5.
+``key_mask`` is bool [batch, kv_len], True = seen; what the masked keys hold does not matter, NaN included
+(keys hidden by causality alone have to be finite: 0 times a NaN among them is a NaN). A query that sees
+no key has output 0, lse minus infinity and no gradient. lse is fp32 [batch, heads, q_len], the natural
+logarithm. ``scale`` defaults to dim ** -0.5.
 
 The backward pass computes the probabilities again from lse; memory grows with the lengths, not with
 their product. Same inputs, same bits: nothing is summed in an order that varies. There is no dropout

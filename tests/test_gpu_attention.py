@@ -186,6 +186,12 @@ def test_flat_and_peaked_rows(dtype, spread):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+def test_scales_of_either_sign(dtype, scale):
+    Case(*tensors(1, 140, 150, 2, 1, 32, dtype, seed=14, spread=0.5), causal=True, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_scores_that_rise_and_fall_along_the_keys(dtype):
     """The running maximum moves at every tile, or only at the first."""
     q, k, v, do = tensors(1, 70, 900, 1, 1, 64, dtype, seed=4)
