@@ -22,6 +22,12 @@
 namespace lsr {
 namespace {
 
+// A lane's row (of 4) and column (of 8) in the warp's tile. Neighbours share a column, and lanes two apart a row, so
+// that of either operand the 16 bytes each that half a warp reads are taken in one pass over the banks (lanes 0-7 in
+// one row instead: 4 x 16 heads x 1024 x 64 causal 357 us forward and 1466 backward, now 333 and 1339).
+__device__ __forceinline__ int lane_row() { return (threadIdx.x & 1) | (threadIdx.x >> 3 & 2); }
+__device__ __forceinline__ int lane_col() { return threadIdx.x >> 1 & 7; }
+
 // out[r][c] = sum_d A[4 r][d] * B[tx + 8 c][d]: A the first of the lane's rows, four apart, B a tile, rows LD
 // apart. Even and odd entries are summed apart, two to an instruction.
 template <int LD, int C>
@@ -197,7 +203,7 @@ __global__ void __launch_bounds__(GTHREADS, 1) attn_fwd_general_kernel(const Att
   extern __shared__ float sm[];
   float *Q = sm, *K = Q + ROWS * LD, *V = K + COLS * LD, *PS = V + COLS * LD, *stat = PS + 8 * 16 * (CW + 4);
   const Place at((p.q_len + ROWS - 1) / ROWS, p.heads);
-  const int warp = threadIdx.x / 32, ty = threadIdx.x % 32 / 8, tx = threadIdx.x % 8, D = p.head_dim;
+  const int warp = threadIdx.x / 32, ty = lane_row(), tx = lane_col(), D = p.head_dim;
   const int i0 = at.tile * ROWS, mine = warp / G * 16 + ty;  // and every fourth row after it
   const int share = warp % G, x0 = share * CW;               // the warp's columns of a tile
   float* P = PS + (warp * 16 + ty) * (CW + 4);
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(GTHREADS, 1) attn_fwd_general_kernel(const Att
         top = fmaxf(top, s[r][c]);
       }
 #pragma unroll
-      for (int w = 4; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      for (int w = 8; w > 1; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
       const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.f : mn;
       const float keep = expf(m[r] - base);
       float sum = 0.f;
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(GTHREADS, 1) attn_fwd_general_kernel(const Att
         P[4 * r * (CW + 4) + tx + 8 * c] = e;
       }
 #pragma unroll
-      for (int w = 4; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      for (int w = 8; w > 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
       l[r] = l[r] * keep + sum;
       m[r] = mn;
 #pragma unroll
@@ -340,7 +346,7 @@ __global__ void __launch_bounds__(GTHREADS, 1) attn_bwd_general_kernel(const Att
   float *PS = SS + 8 * 16 * (CW + 4), *stat = KEYS ? PS + 8 * 16 * (CW + 4) : PS;  // PS: only KEYS multiplies it
   const int rows_len = KEYS ? p.kv_len : p.q_len, cols_len = KEYS ? p.q_len : p.kv_len;
   const Place at((rows_len + ROWS - 1) / ROWS, KEYS ? p.kv_heads : p.heads);
-  const int warp = threadIdx.x / 32, ty = threadIdx.x % 32 / 8, tx = threadIdx.x % 8, D = p.head_dim;
+  const int warp = threadIdx.x / 32, ty = lane_row(), tx = lane_col(), D = p.head_dim;
   const int row0 = at.tile * ROWS, mine = warp / G * 16 + ty;  // and every fourth row after it
   const int share = warp % G, x0 = share * CW;                 // the warp's columns of a tile
   float *P = PS + (warp * 16 + ty) * (CW + 4), *S = SS + (warp * 16 + ty) * (CW + 4);
