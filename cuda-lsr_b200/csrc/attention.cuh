@@ -71,6 +71,12 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+
+// Programmatic dependent launch: the next kernel of the stream may start; wait for the kernel
+// before to have finished and its writes to be seen.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_dependency() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // attention_general.cu: 32-bit arithmetic on the CUDA cores, any type, stride and alignment.
 int attention_forward_general(const AttnParams& p, int dtype, cudaStream_t st);
 int attention_backward_general(const AttnParams& p, int dtype, cudaStream_t st);

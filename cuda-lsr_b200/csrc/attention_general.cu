@@ -145,15 +145,17 @@ __device__ __forceinline__ void store_rows(T* dst, long long stride, int row0, i
   }
 }
 
-// The block's (row tile, head, batch), row tiles fastest.
+// The block's (row tile, head, batch), heads fastest. With a causal rule the tiles that see most come first (the last
+// queries, the first keys), so that short blocks fill the end of the launch.
 struct Place {
   int tile, h, b;
-  __device__ __forceinline__ Place(int tiles, int heads) {
+  __device__ __forceinline__ Place(int tiles, int heads, int batch, bool backwards) {
     unsigned x = blockIdx.x;
-    tile = (int)(x % tiles);
-    x /= tiles;
     h = (int)(x % heads);
-    b = (int)(x / heads);
+    x /= heads;
+    b = (int)(x % batch);
+    tile = (int)(x / batch);
+    if (backwards) tile = tiles - 1 - tile;
   }
 };
 
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(GTHREADS, 1) attn_fwd_general_kernel(const Att
   constexpr int ROWS = L::ROWS, CW = L::CW, COLS = L::COLS, LD = L::LD, CH = DIM / 32, C = CW / 8;
   extern __shared__ float sm[];
   float *Q = sm, *K = Q + ROWS * LD, *V = K + COLS * LD, *PS = V + COLS * LD, *stat = PS + 8 * 16 * (CW + 4);
-  const Place at((p.q_len + ROWS - 1) / ROWS, p.heads);
+  const Place at((p.q_len + ROWS - 1) / ROWS, p.heads, p.batch, true);
   const int warp = threadIdx.x / 32, ty = lane_row(), tx = lane_col(), D = p.head_dim;
   const int i0 = at.tile * ROWS, mine = warp / G * 16 + ty;  // and every fourth row after it
   const int share = warp % G, x0 = share * CW;               // the warp's columns of a tile
@@ -345,7 +347,8 @@ __global__ void __launch_bounds__(GTHREADS, 1) attn_bwd_general_kernel(const Att
   float *R1 = sm, *R2 = R1 + ROWS * LD, *X1 = R2 + ROWS * LD, *X2 = X1 + BUFS * COLS * LD, *SS = X2 + COLS * LD;
   float *PS = SS + 8 * 16 * (CW + 4), *stat = KEYS ? PS + 8 * 16 * (CW + 4) : PS;  // PS: only KEYS multiplies it
   const int rows_len = KEYS ? p.kv_len : p.q_len, cols_len = KEYS ? p.q_len : p.kv_len;
-  const Place at((rows_len + ROWS - 1) / ROWS, KEYS ? p.kv_heads : p.heads);
+  const Place at((rows_len + ROWS - 1) / ROWS, KEYS ? p.kv_heads : p.heads, p.batch, !KEYS);
+  if (KEYS) launch_dependents();
   const int warp = threadIdx.x / 32, ty = lane_row(), tx = lane_col(), D = p.head_dim;
   const int row0 = at.tile * ROWS, mine = warp / G * 16 + ty;  // and every fourth row after it
   const int share = warp % G, x0 = share * CW;                 // the warp's columns of a tile
@@ -467,6 +470,7 @@ __global__ void __launch_bounds__(GTHREADS, 1) attn_bwd_general_kernel(const Att
     store(p.dk, p.sdk, acc2, sc);
   } else {
     store(p.dq, p.sdq, acc2, sc);
+    wait_dependency();  // the launch ends after that of dk and dv
   }
 }
 
@@ -476,16 +480,26 @@ bool vec_ok(const void* base, const AttnStride& s, int batch, int heads, int len
   return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && dim % 4 == 0 && fits(s.b, batch) && fits(s.s, len) && fits(s.h, heads);
 }
 
+// early: blocks start as soon as those of the launch before have all started and leave room.
 template <typename K, typename... A>
-int launch(K kernel, long long blocks, int threads, int smem, cudaStream_t st, A... args) {
+int launch(K kernel, long long blocks, int threads, int smem, cudaStream_t st, bool early, A... args) {
   if (blocks == 0) return LSR_OK;
   if (blocks > 0x7fffffffll) return LSR_ERR_SHAPE;
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return LSR_ERR_LAUNCH;
   ProfScope prof(PK_GEMM_OTHER, st);
-  kernel<<<(unsigned)blocks, threads, smem, st>>>(args...);
-  return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = early;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
 }
 
 // Sets of 16 rows per block: the most whose blocks still fill the SMs.
@@ -500,7 +514,7 @@ int forward_w(const AttnParams& p, bool vec, cudaStream_t st) {
   using L = FwdGeneral<DIM, WR, 8 / WR>;
   static_assert(L::SMEM <= 232448, "shared memory budget exceeded");
   return launch(attn_fwd_general_kernel<T, DIM, WR, 8 / WR>, (long long)cdiv(p.q_len, L::ROWS) * p.heads * p.batch, GTHREADS,
-                L::SMEM, st, p, vec);
+                L::SMEM, st, false, p, vec);
 }
 
 template <typename T, int DIM, int WR, bool KEYS>
@@ -509,7 +523,7 @@ int backward_w(const AttnParams& p, bool vec, cudaStream_t st) {
   static_assert(L::SMEM <= 232448, "shared memory budget exceeded");
   return launch(attn_bwd_general_kernel<T, DIM, WR, 8 / WR, KEYS>,
                 (long long)cdiv(KEYS ? p.kv_len : p.q_len, L::ROWS) * (KEYS ? p.kv_heads : p.heads) * p.batch, GTHREADS,
-                L::SMEM, st, p, vec);
+                L::SMEM, st, !KEYS && p.kv_len > 0, p, vec);
 }
 
 constexpr int least_sets(int dim) { return dim == 64 ? 1 : 2; }  // eight shares of 128 wide tiles do not fit
@@ -537,7 +551,7 @@ int gradients(const AttnParams& p, bool vec, cudaStream_t st) {
 template <typename T, int DIM>
 int backward(const AttnParams& p, bool vec, cudaStream_t st) {
   const long long rows = (long long)p.batch * p.heads * p.q_len;
-  int rc = launch(attn_delta_kernel<T>, (rows + 7) / 8, 256, 0, st, p);
+  int rc = launch(attn_delta_kernel<T>, (rows + 7) / 8, 256, 0, st, false, p);
   if (rc == LSR_OK) rc = gradients<T, DIM, true>(p, vec, st);
   return rc == LSR_OK ? gradients<T, DIM, false>(p, vec, st) : rc;
 }

@@ -60,11 +60,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Programmatic dependent launch: the next kernel of the stream may start its preamble; wait for the kernel
-// before to have finished and its writes to be seen.
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_dependency() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // Give up or take registers, for a whole warpgroup (the block's total stays within what it was launched with).
 template <int N>
 __device__ __forceinline__ void regs_dec() {
