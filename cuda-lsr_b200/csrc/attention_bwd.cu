@@ -15,7 +15,8 @@
 // next are issued as their operands get ready: while the threads take the exponentials of T1, the
 // tensor core adds dS and computes the next T2; while they form dS, it adds P and computes the next T1.
 // Sixteen warps share a tile's scores, 32 columns a thread: with eight the waits on TMEM and on the special
-// function units showed more (4 x 16 heads x 4096 x 64: 1267 us, now 1170, 587 TFLOP/s; dim 128: 1853 us, 742).
+// function units showed more (1267 us to 1170 when changed). 4 x 16 heads x 4096 x 64, no mask: 1134 us, 606 TFLOP/s
+// of the five products; dim 128: 1907 us, 720.
 // P and dS are rounded to 16 bits for the products. In fp16 P is taken times 2^10 (at most 1024), so
 // that rows over thousands of keys stay above its smallest normal value; dV is scaled back.
 #include "attention_sm100.cuh"

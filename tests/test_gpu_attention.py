@@ -124,6 +124,22 @@ def test_many_heads(n, m, d, kv, causal, masked):
     Case(q, k, v, do, causal=causal, key_mask=mask)
 
 
+@pytest.mark.parametrize("causal,masked", [(False, False), (True, True)])
+@pytest.mark.parametrize("d", [64, 65, 96, 97, 128])
+@pytest.mark.parametrize("b,n,m,h,kv", [(2, 300, 200, 40, 40), (1, 150, 260, 40, 8), (1, 100, 300, 16, 2), (1, 70, 300, 3, 1)])
+def test_fp32_with_few_and_many_blocks(b, n, m, h, kv, d, causal, masked):
+    """All divisions of a block's warps among rows and columns, and the widths of a tile."""
+    q, k, v, do = tensors(b, n, m, h, kv, d, torch.float32, seed=n + d)
+    mask = torch.arange(m, device="cuda").expand(b, m) < m - 37 if masked else None
+    Case(q, k, v, do, causal=causal, key_mask=mask)
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("d", [65, 90, 127])
+def test_16_bit_heads_of_odd_widths(dtype, d):
+    Case(*tensors(1, 150, 260, 24, 8, d, dtype, seed=d), causal=True)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("kind", ["right", "left", "holes", "empty entry", "one key", "far tiles"])
@@ -387,3 +403,27 @@ def test_refusals():
     (g,) = torch.autograd.grad(A.attention(x, k, v).float().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.float().sum().backward()
+
+
+def test_fp32_captured_and_replayed_among_other_launches():
+    """The launch that takes dq starts before that of dk and dv has ended: what follows in the stream waits for both."""
+    from lsr import attention as A
+    q, k, v, do = tensors(2, 300, 300, 16, 4, 128, torch.float32, seed=15)
+    out, lse = A.attention_forward(q, k, v, causal=True)
+    want = A.attention_backward(do, q, k, v, out, lse, causal=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        copies = []
+        for _ in range(3):
+            copies.append([t.clone() for t in A.attention_backward(do, q, k, v, out, lse, causal=True)])
+    for _ in range(10):
+        for c in copies:
+            for t in c:
+                t.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for c in copies for x, y in zip(c, want))
+    for _ in range(20):
+        got = A.attention_backward(do, q, k, v, out, lse, causal=True)
+        assert all(torch.equal(x.clone(), y) for x, y in zip(got, want))
