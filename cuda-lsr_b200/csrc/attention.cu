@@ -18,6 +18,15 @@ int check_args(const lsr_attention_args* a) {
   return LSR_OK;
 }
 
+// Whether the tensors are aligned to their entries.
+bool aligned(const lsr_attention_args* a) {
+  const uintptr_t entry = a->dtype == LSR_DTYPE_F32 ? 4 : 2;
+  uintptr_t bits = 0;
+  for (const void* t : {a->q, a->k, a->v, (const void*)a->out, a->dout, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
+    bits |= reinterpret_cast<uintptr_t>(t);
+  return bits % entry == 0 && reinterpret_cast<uintptr_t>(a->lse) % 4 == 0;
+}
+
 AttnStride stride_of(const long long* s) { return AttnStride{s[0], s[1], s[2]}; }
 
 AttnParams params_of(const lsr_attention_args* a) {
@@ -96,6 +105,7 @@ int lsr_attention_forward(const lsr_attention_args* a, void* ws, size_t ws_bytes
   if (rc != LSR_OK) return rc;
   if (a->batch == 0 || a->q_len == 0) return LSR_OK;
   if (!a->q || !a->out || !a->lse || (a->kv_len && (!a->k || !a->v))) return LSR_ERR_ARG;
+  if (!aligned(a)) return LSR_ERR_SHAPE;
   if ((rc = check_device()) != LSR_OK) return rc;
   AttnParams p = params_of(a);
   if (!fast_forward(p, a->dtype)) return attention_forward_general(p, a->dtype, static_cast<cudaStream_t>(stream));
@@ -112,6 +122,7 @@ int lsr_attention_backward(const lsr_attention_args* a, void* ws, size_t ws_byte
   if (a->batch == 0 || (a->q_len == 0 && a->kv_len == 0)) return LSR_OK;
   if (a->q_len && (!a->q || !a->dout || !a->out || !a->lse || !a->dq)) return LSR_ERR_ARG;
   if (a->kv_len && (!a->k || !a->v || !a->dk || !a->dv)) return LSR_ERR_ARG;
+  if (!aligned(a)) return LSR_ERR_SHAPE;
   if (!ws || ws_bytes < lsr_attention_backward_workspace_bytes(a) || (reinterpret_cast<uintptr_t>(ws) & 15))
     return LSR_ERR_WORKSPACE;
   if ((rc = check_device()) != LSR_OK) return rc;

@@ -289,13 +289,17 @@ void sort_spans(Span* s, int n) {
 }
 
 // LSR_OK unless a written range overlaps another tensor's written or read range, or its own read
-// range other than exactly (in place): the blocks run in no order.
+// range other than exactly (in place): the blocks run in no order. The norm is one more read value (given) or
+// written one.
 int check_overlap(const void* const* in, void* const* out, const long long* numel, const int* tin, const int* tout,
-                  int n) {
-  Span* w = static_cast<Span*>(malloc(sizeof(Span) * 2 * (size_t)n));
+                  int n, const float* norm, bool given) {
+  Span* w = static_cast<Span*>(malloc(sizeof(Span) * 2 * ((size_t)n + 1)));
   if (!w) return LSR_ERR_WORKSPACE;
-  Span* r = w + n;
+  Span* r = w + n + 1;
   int nw = 0, nr = 0;
+  const Span at_norm{reinterpret_cast<uintptr_t>(norm), reinterpret_cast<uintptr_t>(norm + 1)};
+  if (given) r[nr++] = at_norm;
+  else w[nw++] = at_norm;
   for (int i = 0; i < n; ++i) {
     if (!numel[i]) continue;
     const uintptr_t a = reinterpret_cast<uintptr_t>(in[i]), b = reinterpret_cast<uintptr_t>(out[i]);
@@ -454,7 +458,7 @@ int lsr_grad_clip(const void* const* grads, void* const* outs, const long long* 
   int rc = check_list(grads, numel, dtypes, count);
   if (rc != LSR_OK) return rc;
   if ((rc = check_list(reinterpret_cast<const void* const*>(outs), numel, out_dtypes, count)) != LSR_OK) return rc;
-  if (count && (rc = check_overlap(grads, outs, numel, dtypes, out_dtypes, count)) != LSR_OK) return rc;
+  if (count && (rc = check_overlap(grads, outs, numel, dtypes, out_dtypes, count, norm, norm_given != 0)) != LSR_OK) return rc;
   if (!norm_given && (!ws || ws_bytes < lsr_grad_workspace_bytes(count))) return LSR_ERR_WORKSPACE;
   if ((rc = check_device()) != LSR_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

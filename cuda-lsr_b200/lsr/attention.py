@@ -16,7 +16,8 @@ logarithm. ``scale`` defaults to dim ** -0.5.
 
 The backward pass computes the probabilities again from lse; memory grows with the lengths, not with
 their product. Same inputs, same bits: nothing is summed in an order that varies. There is no dropout
-and no second derivative. The reference leaves attention to its models' library
+and no second derivative. A captured backward pass wants no eager graph of the same leaves alive
+(PyTorch adds to a leaf's gradient on the stream of the leaf's first graph). The reference leaves attention to its models' library
 (muon_lm_ddp.py:752-822); there is no CPU path: CPU tensors raise ``ValueError``.
 """
 from __future__ import annotations

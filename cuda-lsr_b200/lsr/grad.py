@@ -131,8 +131,9 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
     In place when `out` is None; else out[i] = grads[i] * coefficient in out[i]'s type (same shapes,
     e.g. fp32 gradients to the bf16 that the Muon step takes), and out[i] may be grads[i] itself.
     Apart from that no output may share memory with another output or with a gradient (ValueError).
-    `total_norm`: a 0-d fp32 device tensor to be used instead of computing the norm. A NaN norm makes
-    every entry NaN, an infinite one makes finite entries 0, as torch.nn.utils.clip_grad_norm_ does.
+    `total_norm`: a 0-d fp32 device tensor, not part of an output, to be used instead of computing the norm.
+    A NaN norm makes every entry NaN, an infinite one makes finite entries 0, as
+    torch.nn.utils.clip_grad_norm_ does.
     """
     kind = _kind(norm_type)
     max_norm = float(max_norm)

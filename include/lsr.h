@@ -447,8 +447,9 @@ LSR_API int lsr_coupled_newton_f32(const float* A, float* X, int* iters, float* 
  *   outs[i] may be grads[i] with the same type (in place); otherwise no output
  *   may overlap another output or any input (LSR_ERR_ARG). norm_given = 0: *norm
  *   is computed over these tensors and written; 1: *norm is read (the norm of
- *   more tensors than these, e.g. over all ranks) and ws may be NULL. A NaN
- *   norm makes every output NaN, an infinite one makes finite entries zero.
+ *   more tensors than these, e.g. over all ranks) and ws may be NULL; norm may
+ *   not lie in an output either. A NaN norm makes every output NaN, an infinite
+ *   one makes finite entries zero.
  * ---------------------------------------------------------------------- */
 LSR_API size_t lsr_grad_workspace_bytes(int count);
 LSR_API int lsr_grad_norm(const void* const* grads, const long long* numel, const int* dtypes, int count, int norm_kind,
@@ -477,8 +478,9 @@ LSR_API int lsr_grad_clip(const void* const* grads, void* const* outs, const lon
  * lsr_attention_forward reads q, k, v, key_mask and writes out and lse
  * (fp32 [batch][heads][q_len]); lsr_attention_backward reads those, dout and
  * what the forward pass wrote, and writes dq, dk, dv. No atomics: the same
- * inputs give the same bits. Workspaces are 16-byte aligned; a size of 0 needs
- * none. 16-bit tensors whose addresses, strides and rows are multiples of 16
+ * inputs give the same bits. No output may overlap another tensor of the call.
+ * Tensors are aligned to their entries (LSR_ERR_SHAPE); workspaces are 16-byte
+ * aligned; a size of 0 needs none. 16-bit tensors whose addresses, strides and rows are multiples of 16
  * bytes, with a positive scale, run on the tensor cores; all others in fp32
  * on the CUDA cores.
  * ---------------------------------------------------------------------- */

@@ -138,3 +138,39 @@ def test_driver_flags_and_attention_adapter_refusals():
     assert D._lsr_attention_mask(mask_function=causal_mask_function, attention_mask=m, q_length=3) is m
     with pytest.raises(ValueError):
         D._lsr_attention_mask(mask_function=packed_mask_function, attention_mask=m)
+
+
+@pytest.mark.parametrize("given", [0, 1])
+def test_a_norm_inside_an_output_is_refused(given):
+    from lsr import _lib
+    lib = _lib.load()
+    n, t = array("q", [100, 100]), array("i", [0, 0])
+    ws = ctypes.create_string_buffer(1 << 20)
+
+    def rc(src, dst, norm):
+        src, dst = array("Q", src), array("Q", dst)
+        return lib.lsr_grad_clip(_adr(src), _adr(dst), _adr(n), _adr(t), _adr(t), 2, 2, 1.0, given, norm, ws, 1 << 20, None)
+
+    for at in (4096, 4096 + 396, 8192 + 4):
+        assert rc([4096, 8192], [4096, 8192], at) == -1
+        assert rc([16384, 32768], [4096, 8192], at) == -1
+    if not given:  # the norm would be written over a gradient
+        assert rc([4096, 8192], [16384, 32768], 4100) == -1
+    if not torch.cuda.is_available():
+        assert rc([4096, 8192], [4096, 8192], 4096 + 400) == -6
+        if given:
+            assert rc([4096, 8192], [16384, 32768], 4100) == -6  # a gradient's own entry, only read
+
+
+@pytest.mark.parametrize("dtype,slot,off", [(1, 0, 1), (0, 1, 2), (2, 4, 1), (0, 4, 2), (1, 5, 2), (1, 6, 1), (0, 9, 2)])
+def test_attention_tensors_off_their_entries_are_refused(dtype, slot, off):
+    """slot: of q, k, v, key_mask, out, lse, dout, dq, dk, dv."""
+    import struct
+    from lsr import _lib
+    lib = _lib.load()
+    raw = bytearray(_args(dtype=dtype))
+    at = 40 + 8 * slot
+    assert struct.unpack_from("=Q", raw, at)[0] == 4096
+    struct.pack_into("=Q", raw, at, 4096 + off)
+    assert lib.lsr_attention_backward(bytes(raw), 1 << 20, 1 << 30, None) == -2
+    assert lib.lsr_attention_forward(bytes(raw), 1 << 20, 1 << 30, None) == -2
