@@ -214,7 +214,7 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
                 full + s);
   };
   if (MASK && !KEYS)
-    pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS), mask, tiles, p.a.kv_len, warp, BWD_THREADS / 32, lane);
+    pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS), mask, begin, steps, p.a.kv_len, warp, BWD_THREADS / 32, lane);
   if (warp == ISSUER) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();

@@ -37,9 +37,12 @@ template <int PANELS, int NQ, bool MASK>
 struct FwdSmem {
   static constexpr int TILE = PANELS * kPanel;
   static constexpr int STAGES = NQ == 2 ? (PANELS == 1 ? 8 : 4) : (PANELS == 1 ? 4 : 2);
-  static constexpr int BITS = (NQ + STAGES) * TILE;
-  static constexpr int BARS = BITS + (MASK ? kMaskTiles * 16 : 0);
-  static constexpr int TOTAL = BARS + 256 + 1024;  // and room to align the tiles
+  static constexpr int BARS = (NQ + STAGES) * TILE;
+  static constexpr int BITS = BARS + 256;  // 16 bytes per key tile of the block
+  // With room to align the tiles. A launch asks for the key tiles that it has, so that masked blocks of one query
+  // tile, too, share an SM (3 rows on 4097 keys, 4 x 12 heads: 34 us with room for the longest mask, now 24).
+  static constexpr int total(int tiles) { return BITS + (MASK ? tiles * 16 : 0) + 1024; }
+  static constexpr int TOTAL = total(kMaskTiles);
 };
 
 // Queries [i0, i0 + 128): how many tiles of keys they see, at most.
@@ -115,7 +118,7 @@ __global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1) attn_fwd_kern
     fence_mbar_init();
   }
   if (MASK)
-    pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS), p.a.mask + b * p.a.mask_stride, most, p.a.kv_len, warp,
+    pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS) - first * 4, p.a.mask + b * p.a.mask_stride, first, most, p.a.kv_len, warp,
                   NQ * 4 + 4, lane);
   if (warp == ISSUER) {
     tmem_alloc(tmem_slot, NQ == 2 ? 512 : 256);
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(NQ * 128 + 128, NQ == 1 ? 2 : 1) attn_fwd_kern
   auto s_at = [&](int w) { return tmem + w * 128; };
   auto o_at = [&](int w) { return tmem + NQ * 128 + w * 64 * PANELS; };
   auto p_at = [&](int w) { return APART ? tmem + NQ * 192 + w * 64 : tmem + w * 128; };
-  const KeyBits bits{MASK ? reinterpret_cast<const uint4*>(smem + L::BITS) : nullptr};
+  const KeyBits bits{MASK ? reinterpret_cast<const uint4*>(smem + L::BITS) - first : nullptr};
 
   if (warp >= LOADER) {
     regs_dec<kRestRegs(NQ)>();
@@ -453,7 +456,8 @@ int launch(FwdParams& p, cudaStream_t st) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess)
     return LSR_ERR_LAUNCH;
   ProfScope prof(PK_GEMM_OTHER, st);
-  kernel<<<(unsigned)blocks, NQ * 128 + 128, L::TOTAL, st>>>(p);
+  const int tiles = cdiv(cdiv(p.a.kv_len, kRows), p.splits);  // of a block's share, at most
+  kernel<<<(unsigned)blocks, NQ * 128 + 128, L::total(tiles), st>>>(p);
   return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
 }
 

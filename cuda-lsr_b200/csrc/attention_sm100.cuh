@@ -176,11 +176,11 @@ struct KeyBits {
 };
 constexpr int kMaskTiles = 1536;  // 24 KB of bits: masks of up to 196608 keys
 
-// Every warp packs its share of the mask's bytes for keys [0, min(tiles * 128, len)).
-__device__ __forceinline__ void pack_key_bits(uint32_t* words, const unsigned char* mask, int tiles, int len, int warp,
-                                              int warps, int lane) {
+// Every warp packs its share of the mask's bytes for the key tiles [first, end), as far as there are keys.
+__device__ __forceinline__ void pack_key_bits(uint32_t* words, const unsigned char* mask, int first, int end, int len,
+                                              int warp, int warps, int lane) {
 #pragma unroll 4
-  for (int w = warp; w < tiles * 4; w += warps) {
+  for (int w = first * 4 + warp; w < end * 4; w += warps) {
     const int j = w * 32 + lane;
     const uint32_t v = __ballot_sync(0xffffffffu, j < len && mask[j] != 0);
     if (lane == 0) words[w] = v;
