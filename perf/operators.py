@@ -13,7 +13,6 @@ embedding. `flat` puts the gradients side by side in one buffer, as the bucket v
 Attention cases are [batch, length, heads, dim] with `kv` key heads; `packed` takes queries, keys and values as views of
 one projection's output; `pad` shortens each batch entry's keys with a key mask, and `empty` leaves the last one none.
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -27,7 +26,6 @@ SIZE = {"fp32": 4, "bf16": 2, "fp16": 2}
 ORDER = {"one": 1.0, "two": 2.0, "max": math.inf}  # of the norm
 
 
-@functools.lru_cache(maxsize=None)  # a user's program imports once, not at every call
 def _lsr():
     root = str(Path(__file__).resolve().parent.parent / "cuda-lsr_b200")
     if root not in sys.path:
