@@ -8,7 +8,8 @@
                                                       ``torch.nn.utils.clip_grad_norm_`` is called
 
 The tensors may mix fp32, bf16 and fp16 and any shapes; norms are fp32 device scalars, summed in 64
-bits in one fixed order, and nothing waits for the device unless ``error_if_nonfinite`` is set. The
+bits in one fixed order, and nothing waits for the device unless ``error_if_nonfinite`` is set. Every
+tensor written gets a new version (autograd's check of saved values sees it; a graph's replay does not). The
 list travels in the kernels' parameters, so a call can be captured into a CUDA graph. With gradients
 sharded over ranks: ``grad_norm`` on each rank's own, the ranks' norms combined (for norm 2 the root
 of the sum of squares), then ``clip_grads(..., total_norm=combined)``.
@@ -22,6 +23,7 @@ import math
 from array import array
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -146,6 +148,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
         whole = whole and same
         if list(map(_size_of, dst)) != list(map(_size_of, src)):
             raise ValueError("out must be one tensor of the same shape for each gradient")
+    outs = dst
     if not src:
         return torch.zeros(()) if total_norm is None else total_norm
     first = src[0]
@@ -170,6 +173,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
         _lib.check(rc, "lsr_grad_clip")
         for o, t in back:
             o.copy_(t)
+    # the kernels write through addresses: autograd, and whatever is kept for a tensor's version, is told here
+    increment_version(outs)
     return norm
 
 
