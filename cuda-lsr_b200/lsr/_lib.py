@@ -13,6 +13,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "liblsr.so"
 
@@ -262,3 +263,32 @@ WORKSPACE = Workspace()
 def require_cuda(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (liblsr has no CPU path)")
+
+
+_requires_grad_of = torch.Tensor.requires_grad.__get__
+
+
+def differentiated(tensors) -> bool:
+    """Whether autograd follows any of `tensors` now, backward or forward."""
+    if torch.is_grad_enabled() and any(map(_requires_grad_of, tensors)):
+        return True
+    # (the level says that no forward-mode pass is on without a look at each tensor)
+    return (getattr(forward_ad, "_current_level", 0) >= 0
+            and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
+
+
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, compute, *tensors):
+        ctx.what = what
+        return compute()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} has no gradient: give it detached tensors, or call it under torch.no_grad()")
+
+
+def no_gradient(what: str, compute, tensors):
+    """compute(), a result of `tensors` that has no gradient: where autograd follows them, asking for one raises
+    RuntimeError (NotImplementedError in forward mode at once) instead of counting as zero."""
+    return _NoGradient.apply(what, compute, *tensors) if differentiated(tensors) else compute()

@@ -15,8 +15,9 @@ no key has output 0, lse minus infinity and no gradient. lse is fp32 [batch, hea
 logarithm. ``scale`` defaults to dim ** -0.5.
 
 The backward pass computes the probabilities again from lse; memory grows with the lengths, not with
-their product. Same inputs, same bits: nothing is summed in an order that varies. There is no dropout
-and no second derivative. A captured backward pass wants no eager graph of the same leaves alive
+their product. Same inputs, same bits: nothing is summed in an order that varies. There is no dropout,
+no second derivative and no forward-mode derivative (NotImplementedError); a gradient through the two halves raises
+RuntimeError. A captured backward pass wants no eager graph of the same leaves alive
 (PyTorch adds to a leaf's gradient on the stream of the leaf's first graph). The reference leaves attention to its models' library
 (muon_lm_ddp.py:752-822); there is no CPU path: CPU tensors raise ``ValueError``.
 """
@@ -100,8 +101,7 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def attention_forward(q, k, v, *, causal: bool = False, scale: float | None = None, key_mask=None):
-    """(out, lse): the attention of q over k and v, and the log-sum-exp of each query's scores."""
+def _forward(q, k, v, causal, scale, key_mask):
     _check(q, k, v, key_mask)
     q, k, v, key_mask = _read(q), _read(k), _read(v), _mask(key_mask)
     b, n, h, d = q.shape
@@ -117,8 +117,12 @@ def attention_forward(q, k, v, *, causal: bool = False, scale: float | None = No
     return out, lse
 
 
-def attention_backward(dout, q, k, v, out, lse, *, causal: bool = False, scale: float | None = None, key_mask=None):
-    """(dq, dk, dv) from the output's gradient and what attention_forward returned for the same arguments."""
+def attention_forward(q, k, v, *, causal: bool = False, scale: float | None = None, key_mask=None):
+    """(out, lse): the attention of q over k and v, and the log-sum-exp of each query's scores; no gradient."""
+    return _lib.no_gradient("attention_forward", lambda: _forward(q, k, v, causal, scale, key_mask), (q, k, v))
+
+
+def _backward(dout, q, k, v, out, lse, causal, scale, key_mask):
     _check(q, k, v, key_mask)
     for t, name in ((dout, "dout"), (out, "out")):
         if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
@@ -138,10 +142,16 @@ def attention_backward(dout, q, k, v, out, lse, *, causal: bool = False, scale: 
     return dq, dk, dv
 
 
+def attention_backward(dout, q, k, v, out, lse, *, causal: bool = False, scale: float | None = None, key_mask=None):
+    """(dq, dk, dv) from the output's gradient and what attention_forward returned for the same arguments; no gradient."""
+    return _lib.no_gradient("attention_backward", lambda: _backward(dout, q, k, v, out, lse, causal, scale, key_mask),
+                            (dout, q, k, v, out, lse))
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_mask, causal, scale):
-        out, lse = attention_forward(q, k, v, causal=causal, scale=scale, key_mask=key_mask)
+        out, lse = _forward(q, k, v, causal, scale, key_mask)
         ctx.save_for_backward(q, k, v, key_mask, out, lse)
         ctx.causal, ctx.scale = causal, scale
         return out
@@ -150,15 +160,14 @@ class _Attention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, key_mask, out, lse = ctx.saved_tensors
-        dq, dk, dv = attention_backward(dout, q, k, v, out, lse, causal=ctx.causal, scale=ctx.scale, key_mask=key_mask)
-        return dq, dk, dv, None, None, None
+        return *_backward(dout, q, k, v, out, lse, ctx.causal, ctx.scale, key_mask), None, None, None
 
 
 def attention(q, k, v, *, causal: bool = False, scale: float | None = None, key_mask=None) -> torch.Tensor:
     """The attention of q over k and v, [batch, q_len, heads, dim]; gradients flow to q, k and v."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _lib.differentiated((q, k, v)):
         return _Attention.apply(q, k, v, key_mask, bool(causal), scale)
-    return attention_forward(q, k, v, causal=causal, scale=scale, key_mask=key_mask)[0]
+    return _forward(q, k, v, causal, scale, key_mask)[0]
 
 
 __all__ = ["attention", "attention_forward", "attention_backward"]
