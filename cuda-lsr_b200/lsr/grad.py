@@ -106,11 +106,18 @@ def _flatten(ts, outs):
 
 
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
-    """The norm (1, 2 or inf) over every entry of every tensor: a 0-d fp32 tensor on their device."""
+    """The norm (1, 2 or inf) over every entry of every tensor: a 0-d fp32 tensor on their device.
+
+    It has no gradient: of tensors that autograd follows, the result raises RuntimeError where one is asked of it.
+    """
     kind = _kind(norm_type)
-    ts, ptrs, dtypes, whole = _check_list(tensors, "tensors")
+    ts, *rest = _check_list(tensors, "tensors")
     if not ts:
         return torch.zeros(())
+    return _lib.no_gradient("grad_norm", lambda: _norm(ts, *rest, kind), ts)
+
+
+def _norm(ts, ptrs, dtypes, whole, kind) -> torch.Tensor:
     if not whole:
         ts = [t if _dense(t) else t.detach().contiguous() for t in ts]
         ptrs = array("Q", map(_ptr_of, ts))
@@ -135,7 +142,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
     Apart from that no output may share memory with another output or with a gradient (ValueError).
     `total_norm`: a 0-d fp32 device tensor, not part of an output, to be used instead of computing the norm.
     A NaN norm makes every entry NaN, an infinite one makes finite entries 0, as
-    torch.nn.utils.clip_grad_norm_ does.
+    torch.nn.utils.clip_grad_norm_ does. Like that one it runs without a gradient of its own; forward-mode
+    duals raise NotImplementedError.
     """
     kind = _kind(norm_type)
     max_norm = float(max_norm)
@@ -151,6 +159,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
     outs = dst
     if not src:
         return torch.zeros(()) if total_norm is None else total_norm
+    if _lib.differentiated([*src, *dst] if total_norm is None else [*src, *dst, total_norm]):  # (not backward: no_grad)
+        raise NotImplementedError("clip_grads has no forward-mode derivative")
     first = src[0]
     dev = first.device
     if dst[0].get_device() != first.get_device():

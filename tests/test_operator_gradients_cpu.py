@@ -10,9 +10,12 @@ import torch.autograd.forward_ad as fwd
 @pytest.fixture
 def stub(monkeypatch):
     import lsr.attention as A
+    import lsr.grad as G
     monkeypatch.setattr(A, "_forward", lambda q, k, v, *how: (q.detach() * 2, q.new_zeros(q.shape[0], q.shape[2], q.shape[1])))
     monkeypatch.setattr(A, "_backward", lambda do, q, k, v, *how: (q.detach() * 3, k.detach() * 4, v.detach() * 5))
-    return A
+    monkeypatch.setattr(G, "_check_list", lambda ts, what: (list(ts), [], [], True))
+    monkeypatch.setattr(G, "_norm", lambda ts, *rest: torch.stack([t.detach().square().sum() for t in ts]).sum().sqrt())
+    return A, G
 
 
 def qkv(**how):
@@ -22,30 +25,33 @@ def qkv(**how):
 
 @pytest.mark.parametrize("which", [0, 1, 2])
 @pytest.mark.parametrize("grad_mode", [True, False])
-@pytest.mark.parametrize("name", ["attention", "attention_forward", "attention_backward"])
+@pytest.mark.parametrize("name", ["attention", "attention_forward", "attention_backward", "grad_norm", "clip_grads"])
 def test_forward_mode_is_refused(stub, name, grad_mode, which):
-    A = stub
+    A, G = stub
     with torch.set_grad_enabled(grad_mode), fwd.dual_level():
         ts = qkv()
         ts[which] = fwd.make_dual(ts[which], torch.ones_like(ts[which]))
         call = {"attention": lambda: A.attention(*ts), "attention_forward": lambda: A.attention_forward(*ts),
-                "attention_backward": lambda: A.attention_backward(ts[0], *ts, ts[0], torch.zeros(1, 2, 3))}[name]
+                "attention_backward": lambda: A.attention_backward(ts[0], *ts, ts[0], torch.zeros(1, 2, 3)),
+                "grad_norm": lambda: G.grad_norm(ts), "clip_grads": lambda: G.clip_grads(ts, 1.0)}[name]
         with pytest.raises(NotImplementedError):
             call()
         # duals elsewhere are no concern of the call
         plain = qkv()
-        assert torch.equal(A.attention(*plain), plain[0] * 2)
+        assert torch.equal(A.attention(*plain), plain[0] * 2) and float(G.grad_norm(plain)) > 0
 
 
-@pytest.mark.parametrize("name", ["attention_forward", "attention_backward"])
+@pytest.mark.parametrize("name", ["attention_forward", "attention_backward", "grad_norm"])
 def test_a_gradient_that_is_not_there_raises(stub, name):
-    A = stub
+    A, G = stub
     ts = qkv(grad=True)
 
     def call():
         if name == "attention_forward":
             return A.attention_forward(*ts)[0]
-        return A.attention_backward(ts[0].detach(), *ts, ts[0].detach(), torch.zeros(1, 2, 3))[1]
+        if name == "attention_backward":
+            return A.attention_backward(ts[0].detach(), *ts, ts[0].detach(), torch.zeros(1, 2, 3))[1]
+        return G.grad_norm(ts)
 
     loss = ts[0].square().sum() + call().sum()  # as a penalty beside a loss that has a gradient
     with pytest.raises(RuntimeError, match=name):
@@ -58,7 +64,7 @@ def test_a_gradient_that_is_not_there_raises(stub, name):
 
 
 def test_attention_still_has_its_gradients(stub):
-    A = stub
+    A, _ = stub
     ts = qkv(grad=True)
     A.attention(*ts).sum().backward()
     assert all(torch.equal(t.grad, t.detach() * f) for t, f in zip(ts, (3, 4, 5)))
