@@ -86,16 +86,102 @@ def _address(a: array) -> int:
     return a.buffer_info()[0]
 
 
-def _flatten(ts, outs):
+def _steps(t: torch.Tensor):
+    """[(bytes, most)]: an entry of t lies at its address + sum of bytes * x, 0 <= x <= most, a pair per dimension."""
+    size = t.element_size()
+    return [(st * size, n - 1) for st, n in zip(t.stride(), t.shape) if n > 1]
+
+
+def _reaches(steps, lo: int, hi: int) -> bool:
+    """Whether a sum of bytes * x, 0 <= x <= most over all steps, lies in [lo, hi]. Where that is not settled within
+    10000 trials (strides of no common order), yes."""
+    merged: dict[int, int] = {}
+    for c, n in steps:
+        merged[c] = merged.get(c, 0) + n
+    steps = sorted(merged.items(), reverse=True)
+    rest, common = [0], [0]  # of the steps from k on: their largest sum, and what every sum is a multiple of
+    for c, n in reversed(steps):
+        rest.append(rest[-1] + c * n)
+        common.append(math.gcd(common[-1], c))
+    rest.reverse()
+    common.reverse()
+    left = 10000
+
+    def search(k, lo, hi):
+        nonlocal left
+        if hi < 0 or lo > rest[k]:
+            return False
+        if lo <= 0:
+            return True
+        if k == len(steps) or hi // common[k] * common[k] < lo:
+            return False
+        left -= 1
+        if left < 0:
+            return True
+        c, n = steps[k]
+        return any(search(k + 1, lo - c * x, hi - c * x) for x in range(max(0, -((rest[k + 1] - lo) // c)), min(n, hi // c) + 1))
+
+    return search(0, lo, hi)
+
+
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether an entry of a and one of b have a byte in common."""
+    down = _steps(b)  # counted from b's last entry back
+    apart = a.data_ptr() - b.data_ptr() - sum(c * n for c, n in down)
+    return _reaches(_steps(a) + down, 1 - a.element_size() - apart, b.element_size() - 1 - apart)
+
+
+def _repeats(t: torch.Tensor) -> bool:
+    """Whether two entries of t have a byte in common."""
+    size = t.element_size()
+    steps, span = sorted(_steps(t)), size
+    for c, n in steps:
+        if c < span:
+            break
+        span += c * n
+    else:
+        return False
+    # two different entries: x and y whose first difference is in step k, where it is 1 or more
+    return any(_reaches([(c, n - 1)] + [(d, 2 * m) for d, m in steps[k + 1:]],
+                        1 - size - c + sum(d * m for d, m in steps[k + 1:]), size - 1 - c + sum(d * m for d, m in steps[k + 1:]))
+               for k, (c, n) in enumerate(steps))
+
+
+def _check_shared(grads, outs, norm, checked) -> None:
+    """ValueError where an output shares memory with another, itself, a gradient that it is not, or the norm; `checked`
+    are the numbers of the pairs (gradient, output) that the library compares with one another by itself."""
+    spans = []  # (first byte, end, written, compared by the library, tensor)
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        if not o.numel():
+            continue
+        if i not in checked and _repeats(o):
+            raise ValueError("an output's entries share memory (an expanded tensor, say): clip a copy of it")
+        same = g is o or (g.data_ptr() == o.data_ptr() and g.stride() == o.stride() and g.dtype == o.dtype)
+        for t, written in ((o, True),) if same else ((o, True), (g, False)):
+            spans.append((t.data_ptr(), written, i in checked, t))
+    if norm is not None:
+        spans.append((norm.data_ptr(), False, False, norm))
+    spans = sorted(((at, at + sum(c * n for c, n in _steps(t)) + t.element_size(), w, c, t) for at, w, c, t in spans),
+                   key=lambda x: x[0])
+    open_ = []
+    for x in spans:
+        open_ = [y for y in open_ if y[1] > x[0]]
+        for y in open_:
+            if (x[2] or y[2]) and not (x[3] and y[3]) and _share(x[4], y[4]):
+                raise ValueError("an output shares memory with another output, a gradient or the norm: clip into copies")
+        open_.append(x)
+
+
+def _flatten(ts, outs, norm):
     """(gradients, outputs, [(output, where its values are written first)]) that fill ranges of memory in one order."""
+    direct = {i for i, (t, o) in enumerate(zip(ts, outs)) if _dense(t) and _dense(o) and t.stride() == o.stride()}
+    _check_shared(ts, outs, norm, direct)
     src, dst, back = [], [], []
-    for t, o in zip(ts, outs):
-        if _dense(t) and _dense(o) and t.stride() == o.stride():
+    for i, (t, o) in enumerate(zip(ts, outs)):
+        if i in direct:
             src.append(t)
             dst.append(o)
             continue
-        if any(st == 0 and sz > 1 for st, sz in zip(o.stride(), o.shape)):
-            raise ValueError("an output's entries share memory (an expanded tensor): clip a copy of it")
         src.append(t.detach().contiguous())
         if o.is_contiguous():
             dst.append(o)
@@ -169,7 +255,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
         raise ValueError("total_norm must be one fp32 value on the gradients' device")
     back = []  # (output, dense tensor to copy into it)
     if not whole:
-        src, dst, back = _flatten(src, dst)
+        src, dst, back = _flatten(src, dst, total_norm)
         pin, pout = array("Q", map(_ptr_of, src)), array("Q", map(_ptr_of, dst))
     lib = _lib.load()
     with _lib.on_device(dev):
