@@ -17,7 +17,10 @@
 // Sixteen warps share a tile's scores, 32 columns a thread: with eight the waits on TMEM and on the special
 // function units showed more (1267 us to 1170 when changed). 4 x 16 heads x 4096 x 64, no mask: 1134 us, 606 TFLOP/s
 // of the five products; dim 128: 1907 us, 720.
-// P and dS are rounded to 16 bits for the products (dS of short sequences in two parts, kLowLength). In fp16 P is taken times 2^10 (at most 1024), so
+// P and dS are rounded to 16 bits for the products: half a step of each term, which leaves the gradients with a relative error
+// of 0.0024 in bf16 and 0.0003 in fp16, at 8 keys as at 4096, where the rounding of the results alone makes 0.0017 and
+// 0.0002. A second 16-bit part of dS would bring dq and dk down to that, dv not, for 17.3 us instead of 15.5 at 25
+// heads x 512 x 64. In fp16 P is taken times 2^10 (at most 1024), so
 // that rows over thousands of keys stay above its smallest normal value; dV is scaled back.
 #include "attention_sm100.cuh"
 
@@ -131,7 +134,7 @@ __device__ __forceinline__ void store_part(float* dst, uint32_t at, int col0, in
   }
 }
 
-template <typename T, int PANELS, bool MASK, bool LOW, bool KEYS>
+template <typename T, int PANELS, bool MASK, bool KEYS>
 __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_t* smem) {
   using L = BwdSmem<PANELS, MASK>;
   constexpr int STAGES = L::STAGES;
@@ -308,7 +311,6 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
         if (!wait(ds_ready, pph)) break;
         if (elect_one()) {
           mma_probs<128, COLS, COLS>(acc2, t2, x1, idesc_a, more);
-          if (LOW) mma_probs<128, COLS, COLS>(acc2, t2 + COLS / 2, x1, idesc_a, 1);
           umma_commit(left);
           if (jn < steps) scores2();
         }
@@ -416,18 +418,8 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
                x[3]);
         pr[e / 2] = pack2<T>(x[0], x[1]);
         pr[e / 2 + 1] = pack2<T>(x[2], x[3]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) d[e + k] = __float_as_uint(x[k]);
       }
       tmem_st16(my2, pr);
-      if (LOW) {  // what the rounding left, beside it
-#pragma unroll
-        for (int e = 0; e < COLS / 2; ++e) {
-          const float2 hi = unpack2<T>(pr[e]);
-          pr[e] = pack2<T>(__uint_as_float(d[2 * e]) - hi.x, __uint_as_float(d[2 * e + 1]) - hi.y);
-        }
-        tmem_st16(my2 + COLS / 2, pr);
-      }
       if (MASK && !KEYS) {  // nor what its keys hold
         const uint32_t seen = reinterpret_cast<const uint32_t*>(bits.bits + j)[r / 32];
         if (!((seen >> lane) & 1) && part < PANELS) {
@@ -478,12 +470,12 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
   }
 }
 
-template <typename T, int PANELS, bool MASK, bool LOW>
+template <typename T, int PANELS, bool MASK>
 __global__ void __launch_bounds__(BWD_THREADS, 1) attn_bwd_kernel(const __grid_constant__ BwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;
-  if (blockIdx.x < p.kv_blocks) bwd_block<T, PANELS, MASK, LOW, true>(p, blockIdx.x, smem);
-  else bwd_block<T, PANELS, MASK, LOW, false>(p, blockIdx.x - (unsigned)p.kv_blocks, smem);
+  if (blockIdx.x < p.kv_blocks) bwd_block<T, PANELS, MASK, true>(p, blockIdx.x, smem);
+  else bwd_block<T, PANELS, MASK, false>(p, blockIdx.x - (unsigned)p.kv_blocks, smem);
 }
 
 // The sums of several blocks added in order and rounded, a warp per row of dq, dk or dv.
@@ -515,7 +507,7 @@ __global__ void __launch_bounds__(256) attn_join_grads_kernel(const __grid_const
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(x[0] * mul, x[1] * mul), pack2<T>(x[2] * mul, x[3] * mul));
 }
 
-template <typename T, int PANELS, bool MASK, bool LOW>
+template <typename T, int PANELS, bool MASK>
 int launch(BwdParams& p, cudaStream_t st) {
   using L = BwdSmem<PANELS, MASK>;
   static_assert(L::TOTAL <= 232448, "shared memory budget exceeded");
@@ -527,7 +519,7 @@ int launch(BwdParams& p, cudaStream_t st) {
     attn_stats_kernel<T><<<(unsigned)(rows / 32), 256, 0, st>>>(p);
     if (cudaGetLastError() != cudaSuccess) return LSR_ERR_LAUNCH;
   }
-  auto kernel = attn_bwd_kernel<T, PANELS, MASK, LOW>;
+  auto kernel = attn_bwd_kernel<T, PANELS, MASK>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL) != cudaSuccess)
     return LSR_ERR_LAUNCH;
   {
@@ -559,12 +551,6 @@ int split_count(long long steps, long long mean) {
   return 2 * steps >= 3 * mean ? (int)std::min<long long>((steps + mean - 1) / mean, 64) : 1;
 }
 
-// Short sequences have rows of few keys, whose dS are differences of near values, and few terms over which their
-// rounding would average out: there dS is multiplied in two parts, the rounded value and what that left (64 queries
-// and keys, causal, bf16: dq's relative error 0.0020, 0.0025 in one part, 0.0016 rounded from the exact value). Longer
-// ones go without: 25 heads x 512 x 64 take 17.6 us, 15.5 in one part.
-constexpr int kLowLength = 512;
-
 void set_splits(BwdParams& p) {
   p.q_tiles = cdiv(p.a.q_len, kRows);
   p.kv_tiles = cdiv(p.a.kv_len, kRows);
@@ -575,15 +561,10 @@ void set_splits(BwdParams& p) {
   p.split_q = split_count(q_steps, mean);
 }
 
-template <typename T, int PANELS, bool MASK>
-int launch_low(BwdParams& p, cudaStream_t st) {
-  return std::min(p.a.q_len, p.a.kv_len) <= kLowLength ? launch<T, PANELS, MASK, true>(p, st) : launch<T, PANELS, MASK, false>(p, st);
-}
-
 template <typename T>
 int backward(BwdParams& p, cudaStream_t st) {
-  if (p.a.head_dim > 64) return p.a.mask ? launch_low<T, 2, true>(p, st) : launch_low<T, 2, false>(p, st);
-  return p.a.mask ? launch_low<T, 1, true>(p, st) : launch_low<T, 1, false>(p, st);
+  if (p.a.head_dim > 64) return p.a.mask ? launch<T, 2, true>(p, st) : launch<T, 2, false>(p, st);
+  return p.a.mask ? launch<T, 1, true>(p, st) : launch<T, 1, false>(p, st);
 }
 
 }  // namespace
