@@ -95,7 +95,7 @@ size_t lsr_attention_backward_workspace_bytes(const lsr_attention_args* a) {
   using namespace lsr;
   if (check_args(a) != LSR_OK || a->batch == 0) return 0;
   const AttnParams p = params_of(a);
-  if (fast_backward(p, a->dtype)) return attention_backward_sm100_ws(p);
+  if (fast_backward(p, a->dtype)) return attention_backward_sm100_ws(p, a->dtype);
   return (size_t)a->batch * a->heads * a->q_len * sizeof(float) + 16;
 }
 

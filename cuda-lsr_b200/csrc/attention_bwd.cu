@@ -21,7 +21,13 @@
 // of 0.0024 in bf16 and 0.0003 in fp16, at 8 keys as at 4096, where the rounding of the results alone makes 0.0017 and
 // 0.0002. A second 16-bit part of dS would bring dq and dk down to that, dv not, for 17.3 us instead of 15.5 at 25
 // heads x 512 x 64. In fp16 P is taken times 2^10 (at most 1024), so
-// that rows over thousands of keys stay above its smallest normal value; dV is scaled back.
+// that rows over thousands of keys stay above its smallest normal value; dV is scaled back. dS has no size of its own
+// (loss-scaled gradients pass fp16's largest value, small ones over many keys lie among its smallest), so in fp16
+// it is taken times 2^x, one x for a key head and the query heads that share it, from
+//   |dS| <= |dO_i| (max |v_j| + |o_i|) <= B = 2 max |dO_i| max |v_j|,   2^13 <= 2^x B < 2^14,
+// over the rows that are seen and finite: nothing overflows, and what is lost lies 2^-38 below B. The kernel that takes D
+// leaves the largest of each tile, and every block takes the largest of those again (8 x 16 heads x 1024 x 64 causal: 144.7 us,
+// 143.6 without; dS unscaled lost a tenth of dq at dout of 1e-4 on 8192 keys, and made NaN of dP beyond 2^17).
 #include "attention_sm100.cuh"
 
 namespace lsr {
@@ -29,10 +35,16 @@ namespace {
 
 constexpr int PARTS = 4;  // warpgroups on the scores, each with 128 / PARTS columns
 constexpr int COLS = kRows / PARTS;
-constexpr int BWD_THREADS = PARTS * 128 + 128;  // then the loader, the issuer and two idle warps
-constexpr int LOADER = 4 * PARTS, ISSUER = LOADER + 1;
+constexpr int BWD_THREADS = PARTS * 128 + 128;  // then the loader, the issuer, one for the size of dS (kSized) and an idle warp
+constexpr int LOADER = 4 * PARTS, ISSUER = LOADER + 1, SIZER = ISSUER + 1;
 // Registers a thread after the split, within the 96 that five warpgroups are launched with: 5 x 96 = 4 x 104 + 64.
 constexpr int kScoreRegs = 104, kRestRegs = 64;
+
+// Whether dS is scaled to a size of the data.
+template <typename T>
+constexpr bool kSized = false;
+template <>
+constexpr bool kSized<__half> = true;
 
 // Extra power of two in P.
 template <typename T>
@@ -43,7 +55,11 @@ constexpr int kExtra<__half> = 10;
 struct BwdParams {
   AttnParams a;
   CUtensorMap mq, mk, mv, mdo;
-  float* stats;  // [batch][heads][query tiles][2][128]: lse log2 e - extra (plus infinity: no probability), D 2^-extra
+  float* stats;  // [batch][heads][query tiles][2][128]: lse log2 e - extra (plus infinity: no probability), D
+  // kSized: the largest |dout row|^2 of each tile, [batch][heads][q_tiles], then the largest |v row|^2 among its keys that are
+  // seen, [batch][kv_heads][kv_tiles]; rows that are not finite do not count
+  float* sizes;
+  long long size_rows;  // query tiles
   int q_tiles, kv_tiles;
   long long kv_blocks;
   // blocks that the steps of 128 keys, and of 128 queries, are dealt to; with more than one their sums go here
@@ -61,34 +77,107 @@ struct BwdSmem {
   static constexpr int TOTAL = BARS + 256 + 1024;  // and room to align the tiles
 };
 
-// Row statistics, eight lanes per row.
+template <typename T>
+__device__ __forceinline__ float dot8(const uint4& x, const uint4& y, float s) {
+  const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s = fmaf(attn_to_f(xe[k]), attn_to_f(ye[k]), s);
+  return s;
+}
+
+// A sum over the eight lanes of a row.
+__device__ __forceinline__ float row_sum(float s) {
+#pragma unroll
+  for (int w = 4; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+  return s;
+}
+
+// Row statistics: a tile of 128 rows per block, eight lanes per row, four rows per thread in flight (one row per thread and
+// 32 per block: 23.5 us at 8 x 16 heads x 1024 x 64 in fp16, now 12.8). kSized: the blocks after those of the
+// queries take the sizes of the values.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ BwdParams p) {
   launch_dependents();
-  const long long row = (long long)blockIdx.x * 32 + threadIdx.x / 8;  // rows of whole tiles
-  const int len = p.q_tiles * kRows, part = threadIdx.x % 8;
-  const int i = (int)(row % len), h = (int)(row / len % p.a.heads), b = (int)(row / len / p.a.heads);
-  if (b >= p.a.batch) return;
-  float s = 0.f, lse = INFINITY;
-  if (i < p.a.q_len) {
-    const T* o = attn_at<T>(p.a.out, p.a.so, b, h) + i * p.a.so.s;
-    const T* d = attn_at<T>(p.a.dout, p.a.sdo, b, h) + i * p.a.sdo.s;
+  const bool keys = kSized<T> && blockIdx.x >= p.size_rows;
+  const long long id = blockIdx.x - (keys ? p.size_rows : 0);
+  const int tiles = keys ? p.kv_tiles : p.q_tiles, heads = keys ? p.a.kv_heads : p.a.heads;
+  const int part = threadIdx.x % 8, sub = threadIdx.x / 8;
+  const int row0 = (int)(id % tiles) * kRows + sub, h = (int)(id / tiles % heads), b = (int)(id / tiles / heads);
+  float s[4] = {}, z[4] = {};  // dout . out (not of keys), and the row's own square (kSized)
+  if (keys) {
+    const T* v = attn_at<T>(p.a.v, p.a.sv, b, h);
+    const unsigned char* mask = p.a.mask ? p.a.mask + b * p.a.mask_stride : nullptr;
     for (int e = part * 8; e < p.a.head_dim; e += 64) {
-      const uint4 x = *reinterpret_cast<const uint4*>(o + e), y = *reinterpret_cast<const uint4*>(d + e);
-      const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y);
+      uint4 x[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s = fmaf(attn_to_f(xe[k]), attn_to_f(ye[k]), s);
+      for (int k = 0; k < 4; ++k) {
+        const int j = row0 + 32 * k;
+        x[k] = j < p.a.kv_len && (!mask || mask[j]) ? *reinterpret_cast<const uint4*>(v + j * p.a.sv.s + e) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[k] = dot8<T>(x[k], x[k], z[k]);
     }
-    const float v = p.a.lse[((long long)b * p.a.heads + h) * p.a.q_len + i];
-    if (v != -INFINITY) lse = fmaf(v, kLog2e, -(float)kExtra<T>);
-  }
+  } else {
+    const T *o = attn_at<T>(p.a.out, p.a.so, b, h), *d = attn_at<T>(p.a.dout, p.a.sdo, b, h);
+    const float* from = p.a.lse + ((long long)b * p.a.heads + h) * p.a.q_len;
+    float lse[4];
 #pragma unroll
-  for (int w = 4; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-  if (part == 0) {
-    float* dst = p.stats + row / kRows * 256 + row % kRows;
-    dst[0] = lse;
-    dst[128] = s * (1.f / (1 << kExtra<T>));
+    for (int k = 0; k < 4; ++k) lse[k] = row0 + 32 * k < p.a.q_len ? from[row0 + 32 * k] : -INFINITY;
+    for (int e = part * 8; e < p.a.head_dim; e += 64) {
+      uint4 x[4], y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = row0 + 32 * k;
+        const bool in = i < p.a.q_len;
+        x[k] = in ? *reinterpret_cast<const uint4*>(o + i * p.a.so.s + e) : make_uint4(0, 0, 0, 0);
+        y[k] = in ? *reinterpret_cast<const uint4*>(d + i * p.a.sdo.s + e) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        s[k] = dot8<T>(x[k], y[k], s[k]);
+        if (kSized<T>) z[k] = dot8<T>(y[k], y[k], z[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float delta = row_sum(s[k]);
+      if (part == 0) {
+        float* dst = p.stats + id * 256 + sub + 32 * k;
+        dst[0] = lse[k] != -INFINITY ? fmaf(lse[k], kLog2e, -(float)kExtra<T>) : INFINITY;
+        dst[128] = delta;
+      }
+    }
   }
+  if (!kSized<T>) return;
+  __shared__ unsigned tops[8];
+  unsigned top = 0;  // of the finite ones: values >= 0 are ordered as their bits are
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float x = row_sum(z[k]);
+    top = max(top, x < INFINITY ? __float_as_uint(x) : 0u);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+  __syncthreads();
+  if (threadIdx.x) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) top = max(top, tops[w]);
+  p.sizes[blockIdx.x] = __uint_as_float(top);
+}
+
+// The power of two that dS of a key head is taken times, the same for a whole warp.
+template <typename T>
+__device__ __forceinline__ float ds_scale(const BwdParams& p, int b, int hk, int lane) {
+  if (!kSized<T>) return 1.f;
+  const long long at = (long long)b * p.a.kv_heads + hk, rows = (long long)p.q_tiles * p.a.group, keys = p.kv_tiles;
+  const float *of_rows = p.sizes + at * rows, *of_keys = p.sizes + p.size_rows + at * keys;
+  unsigned d2 = 0, v2 = 0;
+  for (long long k = lane; k < rows; k += 32) d2 = max(d2, __float_as_uint(of_rows[k]));
+  for (long long k = lane; k < keys; k += 32) v2 = max(v2, __float_as_uint(of_keys[k]));
+  const float bound = 2.f * sqrtf(__uint_as_float(__reduce_max_sync(0xffffffffu, d2))) *
+                      sqrtf(__uint_as_float(__reduce_max_sync(0xffffffffu, v2)));
+  // 2^-47 to 2^41, or 0
+  return bound > 0.f ? __uint_as_float((2 * 127 + 13 - (__float_as_uint(bound) >> 23)) << 23) : 1.f;
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -120,8 +209,8 @@ __device__ __forceinline__ void store_rows(T* dst, uint32_t at, int col0, int co
   }
 }
 
-// The same in 32 bits, as it is.
-__device__ __forceinline__ void store_part(float* dst, uint32_t at, int col0, int col1, int dim, bool live, bool any) {
+// The same in 32 bits.
+__device__ __forceinline__ void store_part(float* dst, uint32_t at, int col0, int col1, int dim, bool live, bool any, float mul) {
   for (int q = col0; q < col1; q += 32) {
     uint32_t o[32];
     tmem_ld32(at + q, o);
@@ -129,8 +218,10 @@ __device__ __forceinline__ void store_part(float* dst, uint32_t at, int col0, in
 #pragma unroll
     for (int e = 0; e < 32; e += 4)
       if (live && q + e < dim)
-        *reinterpret_cast<uint4*>(dst + q + e) =
-            any ? make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<float4*>(dst + q + e) =
+            any ? make_float4(__uint_as_float(o[e]) * mul, __uint_as_float(o[e + 1]) * mul, __uint_as_float(o[e + 2]) * mul,
+                              __uint_as_float(o[e + 3]) * mul)
+                : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
@@ -141,9 +232,10 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
   uint8_t *r1 = smem, *r2 = smem + L::TILE, *ring = smem + 2 * L::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
   uint64_t *fixed = bars, *full = fixed + 1, *empty = full + STAGES, *t1_full = empty + STAGES, *t2_full = t1_full + 1,
-           *p_ready = t2_full + 1, *ds_ready = p_ready + 1, *done = ds_ready + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+           *p_ready = t2_full + 1, *ds_ready = p_ready + 1, *done = ds_ready + 1, *sized = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sized + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* size_slot = reinterpret_cast<float*>(tmem_slot + 2);
   // the same in all lanes, and known to be: the roles below then run as uniform code
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int off = p.a.kv_len - p.a.q_len;  // under causality query i sees keys up to i + off
@@ -186,6 +278,7 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
     mbar_init(p_ready, 4 * PARTS);
     mbar_init(ds_ready, 4 * PARTS);
     mbar_init(done, 1);
+    mbar_init(sized, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -330,6 +423,13 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
           break;
         }
       __syncwarp();
+    } else if (kSized<T> && warp == SIZER) {
+      wait_dependency();
+      const float up = ds_scale<T>(p, b, KEYS ? h : h / p.a.group, lane);
+      if (lane == 0) {
+        *size_slot = up;
+        mbar_arrive(sized);
+      }
     }
   } else {
     regs_inc<kScoreRegs>();
@@ -347,9 +447,10 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
       wait_dependency();
       const float* st = p.stats + (((long long)b * p.a.heads + h) * p.q_tiles + tile) * 256 + r;
       lse = st[0] + (float)kExtra<T>;
-      delta = st[128] * (float)(1 << kExtra<T>);
+      delta = st[128];
     }
-    for (int j = start; j < steps; j = bits.next(j + 1, steps)) {
+    if (kSized<T>) ok = warp_wait(sized, 0, abort_flag, status, ST_ATTN_SOFTMAX);
+    for (int j = start; ok && j < steps; j = bits.next(j + 1, steps)) {
       const int t0 = (KEYS ? first + j % tiles : j) * kRows + part * COLS;  // position of the thread's first column
       // the statistics come with the step's first tile
       if (KEYS && !(ok = warp_wait(full + cur, sph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
@@ -404,18 +505,17 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
         for (int e = 0; e < COLS; ++e)
           if (!((word >> e) & 1)) d[e] = 0;
       }
-      constexpr float kDown = 1.f / (1 << (KEYS ? kExtra<T> : 0));
-      const uint64_t down = pair(kDown, kDown);
+      // kSized: P times 2^x (read again in every step: there are no registers to spare), and without its extra power
+      const float up = kSized<T> ? *size_slot : 1.f;
+      const uint64_t by = pair(up * (1.f / (1 << (KEYS ? kExtra<T> : 0))), up * (1.f / (1 << (KEYS ? kExtra<T> : 0))));
 #pragma unroll
       for (int e = 0; e < COLS; e += 4) {
         const float4 v = KEYS ? stat[32 + e / 4] : make_float4(delta, delta, delta, delta);
-        const uint64_t a0 = pair(__uint_as_float(d[e]), __uint_as_float(d[e + 1]));
-        const uint64_t a1 = pair(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3]));
-        const uint64_t m0 = pair(-v.x, -v.y), m1 = pair(-v.z, -v.w);
+        uint64_t p0 = pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), p1 = pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+        if (kSized<T>) p0 = mul2(p0, by), p1 = mul2(p1, by);
         float x[4];
-        unpair(mul2(kDown == 1.f ? add2(a0, m0) : fma2(a0, down, m0), pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1]))), x[0], x[1]);
-        unpair(mul2(kDown == 1.f ? add2(a1, m1) : fma2(a1, down, m1), pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]))), x[2],
-               x[3]);
+        unpair(mul2(add2(pair(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), pair(-v.x, -v.y)), p0), x[0], x[1]);
+        unpair(mul2(add2(pair(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])), pair(-v.z, -v.w)), p1), x[2], x[3]);
         pr[e / 2] = pack2<T>(x[0], x[1]);
         pr[e / 2 + 1] = pack2<T>(x[2], x[3]);
       }
@@ -439,6 +539,7 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
     tc_fence_after();
     if (ok) {
       const bool any = start < steps && !dead_key;
+      const float back = kSized<T> ? 1.f / *size_slot : 1.f;
       constexpr int SHARE = 64 * PANELS / (PARTS / 2);  // half of the warpgroups store dv, half dk
       const bool second = part >= PARTS / 2;
       const int col = part % (PARTS / 2) * SHARE;
@@ -446,8 +547,9 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
         const int len = KEYS ? p.a.kv_len : p.a.q_len, heads = KEYS ? p.a.kv_heads : p.a.heads;
         float* to = (KEYS ? (second ? p.part_dk : p.part_dv) : p.part_dq) +
                     ((((long long)split * p.a.batch + b) * heads + h) * len + row) * p.a.head_dim;
-        if (KEYS) store_part(to, (second ? acc2 : acc1) + quarter, col, col + SHARE, p.a.head_dim, row < len, any);
-        else if (part < 2 * PANELS) store_part(to, acc2 + quarter, part * 32, part * 32 + 32, p.a.head_dim, row < len, any);
+        if (KEYS) store_part(to, (second ? acc2 : acc1) + quarter, col, col + SHARE, p.a.head_dim, row < len, any,
+                             second ? back : 1.f);
+        else if (part < 2 * PANELS) store_part(to, acc2 + quarter, part * 32, part * 32 + 32, p.a.head_dim, row < len, any, back);
       } else if (KEYS) {
         const bool live = row < p.a.kv_len;
         if (!second)
@@ -455,10 +557,10 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
                      1.f / (1 << kExtra<T>));
         else
           store_rows(attn_at<T>(p.a.dk, p.a.sdk, b, h) + row * p.a.sdk.s, acc2 + quarter, col, col + SHARE, p.a.head_dim, live, any,
-                     p.a.scale);
+                     p.a.scale * back);
       } else if (part < 2 * PANELS) {
         store_rows(attn_at<T>(p.a.dq, p.a.sdq, b, h) + row * p.a.sdq.s, acc2 + quarter, part * 32, part * 32 + 32, p.a.head_dim,
-                   row < p.a.q_len, any, p.a.scale);
+                   row < p.a.q_len, any, p.a.scale * back);
       }
     }
   }
@@ -511,12 +613,12 @@ template <typename T, int PANELS, bool MASK>
 int launch(BwdParams& p, cudaStream_t st) {
   using L = BwdSmem<PANELS, MASK>;
   static_assert(L::TOTAL <= 232448, "shared memory budget exceeded");
-  const long long rows = (long long)p.q_tiles * kRows * p.a.heads * p.a.batch;
   const long long blocks = p.kv_blocks + (long long)p.q_tiles * p.a.heads * p.a.batch * p.split_q;
-  if (blocks > 0x7fffffffll || rows / 32 > 0x7fffffffll) return LSR_ERR_SHAPE;
+  const long long stat_blocks = p.size_rows + (kSized<T> ? (long long)p.kv_tiles * p.a.kv_heads * p.a.batch : 0);
+  if (blocks > 0x7fffffffll || stat_blocks > 0x7fffffffll) return LSR_ERR_SHAPE;
   {
     ProfScope prof(PK_EW_OTHER, st);
-    attn_stats_kernel<T><<<(unsigned)(rows / 32), 256, 0, st>>>(p);
+    attn_stats_kernel<T><<<(unsigned)stat_blocks, 256, 0, st>>>(p);
     if (cudaGetLastError() != cudaSuccess) return LSR_ERR_LAUNCH;
   }
   auto kernel = attn_bwd_kernel<T, PANELS, MASK>;
@@ -567,13 +669,19 @@ int backward(BwdParams& p, cudaStream_t st) {
   return p.a.mask ? launch<T, 1, true>(p, st) : launch<T, 1, false>(p, st);
 }
 
+// Entries of BwdParams::sizes, rounded up so that 16-byte alignment goes on.
+size_t size_count(const BwdParams& p, int dtype) {
+  const size_t n = ((size_t)p.q_tiles * p.a.heads + (size_t)p.kv_tiles * p.a.kv_heads) * p.a.batch;
+  return dtype == LSR_DTYPE_F16 ? (n + 3) / 4 * 4 : 0;
+}
+
 }  // namespace
 
-size_t attention_backward_sm100_ws(const AttnParams& a) {
+size_t attention_backward_sm100_ws(const AttnParams& a, int dtype) {
   BwdParams p{};
   p.a = a;
   set_splits(p);
-  size_t floats = (size_t)p.q_tiles * a.heads * a.batch * 256;
+  size_t floats = (size_t)p.q_tiles * a.heads * a.batch * 256 + size_count(p, dtype);
   if (p.split_k > 1) floats += (size_t)p.split_k * 2 * a.batch * a.kv_heads * a.kv_len * a.head_dim;
   if (p.split_q > 1) floats += (size_t)p.split_q * a.batch * a.heads * a.q_len * a.head_dim;
   return floats * sizeof(float);
@@ -584,7 +692,9 @@ int attention_backward_sm100(const AttnParams& a, int dtype, void* ws, cudaStrea
   p.a = a;
   set_splits(p);
   p.stats = static_cast<float*>(ws);
-  p.part_dk = p.stats + (size_t)p.q_tiles * a.heads * a.batch * 256;
+  p.size_rows = (long long)p.q_tiles * a.heads * a.batch;
+  p.sizes = p.stats + (size_t)p.q_tiles * a.heads * a.batch * 256;
+  p.part_dk = p.sizes + size_count(p, dtype);
   const size_t kv = p.split_k > 1 ? (size_t)p.split_k * a.batch * a.kv_heads * a.kv_len * a.head_dim : 0;
   p.part_dv = p.part_dk + kv;
   p.part_dq = p.part_dv + kv;

@@ -195,6 +195,6 @@ bool rows_ok(const void* base, const AttnStride& s, int batch, int heads, int le
 int attention_forward_sm100(const AttnParams& p, int dtype, void* ws, cudaStream_t st);
 size_t attention_forward_sm100_ws(const AttnParams& p);
 int attention_backward_sm100(const AttnParams& p, int dtype, void* ws, cudaStream_t st);
-size_t attention_backward_sm100_ws(const AttnParams& p);
+size_t attention_backward_sm100_ws(const AttnParams& p, int dtype);
 
 }  // namespace lsr

@@ -474,7 +474,10 @@ LSR_API int lsr_grad_clip(const void* const* grads, void* const* outs, const lon
  * of k and v hold does not matter, NaN included. head_dim 1..128; strides in
  * elements (batch, position, head), the head_dim entries of a head contiguous.
  * Probabilities and sums are fp32; with 16-bit types p and ds are rounded to
- * that type as operands of the products that take them, whatever the lengths.
+ * that type as operands of the products that take them, whatever the lengths. In
+ * fp16 ds is brought to its range by a power of two of the data first: it loses
+ * at most 2^-38 of 2 max |dout_i| max |v_j| of its key head beside the rounding,
+ * and overflows only where the gradients themselves do.
  * lsr_attention_forward reads q, k, v, key_mask and writes out and lse
  * (fp32 [batch][heads][q_len]); lsr_attention_backward reads those, dout and
  * what the forward pass wrote, and writes dq, dk, dv. No atomics: the same
