@@ -65,7 +65,7 @@ AttnParams params_of(const lsr_attention_args* a) {
 // The tensor-core kernels read by TMA: 16-bit types, 16-byte addresses, strides and rows. They take the
 // row maximum of unscaled scores, which is that of the scaled ones for a positive scale.
 bool fast_forward(const AttnParams& p, int dtype) {
-  return dtype != LSR_DTYPE_F32 && p.scale > 0.f && p.kv_len > 0 && (!p.mask || p.kv_len <= kMaskTiles * kRows) &&
+  return dtype != LSR_DTYPE_F32 && p.scale > 0.f && p.kv_len > 0 &&
          rows_ok(p.q, p.sq, p.batch, p.heads, p.q_len, p.head_dim) &&
          rows_ok(p.k, p.sk, p.batch, p.kv_heads, p.kv_len, p.head_dim) &&
          rows_ok(p.v, p.sv, p.batch, p.kv_heads, p.kv_len, p.head_dim) &&

@@ -310,7 +310,7 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
                 full + s);
   };
   if (MASK && !KEYS)
-    pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS), mask, begin, steps, p.a.kv_len, warp, BWD_THREADS / 32, lane);
+    pack_key_bits(reinterpret_cast<uint32_t*>(smem + L::BITS) - begin * 4, mask, begin, steps, p.a.kv_len, warp, BWD_THREADS / 32, lane);
   if (warp == ISSUER) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -329,7 +329,7 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
   }
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, t1 = tmem, t2 = tmem + 128, acc1 = tmem + 256, acc2 = tmem + 256 + 64 * PANELS;
-  const KeyBits bits{MASK && !KEYS ? reinterpret_cast<const uint4*>(smem + L::BITS) : nullptr};
+  const KeyBits bits{MASK && !KEYS ? reinterpret_cast<const uint4*>(smem + L::BITS) - begin : nullptr};
   const int start = bits.next(begin, steps);
 
   if (warp >= LOADER) {
@@ -660,7 +660,7 @@ void set_splits(BwdParams& p) {
   const long long q_sets = (long long)p.q_tiles * p.a.heads * p.a.batch, q_steps = p.kv_tiles;
   const long long sms = device_sm_count(), mean = (k_sets * k_steps + q_sets * q_steps + sms - 1) / sms;
   p.split_k = split_count(k_steps, mean);
-  p.split_q = split_count(q_steps, mean);
+  p.split_q = std::max(split_count(q_steps, mean), mask_splits(p.a));
 }
 
 template <typename T>

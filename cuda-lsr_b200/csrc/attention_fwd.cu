@@ -473,11 +473,12 @@ int query_tiles(const AttnParams& p) {
 }
 
 // Blocks that the key tiles of a block's queries are dealt to when there are few queries: as many as
-// the SMs have room for, with four tiles each at least, so that the join does not cost more than it saves.
+// the SMs have room for, with four tiles each at least, so that the join does not cost more than it saves. And as many
+// as a long mask's bits take.
 int split_count(const AttnParams& p) {
   const long long blocks = (long long)cdiv(p.q_len, query_tiles(p) * kRows) * p.heads * p.batch;
   const int tiles = cdiv(p.kv_len, kRows), room = 2 * device_sm_count();
-  return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(room / blocks, tiles / 4), 64));
+  return (int)std::max<long long>(mask_splits(p), std::min<long long>(std::min<long long>(room / blocks, tiles / 4), 64));
 }
 
 template <typename T>

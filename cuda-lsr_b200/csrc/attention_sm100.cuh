@@ -174,7 +174,8 @@ struct KeyBits {
     return j;
   }
 };
-constexpr int kMaskTiles = 1536;  // 24 KB of bits: masks of up to 196608 keys
+constexpr int kMaskTiles = 1536;  // that a block has room for, 24 KB of bits: of more than 196608 masked keys each block takes a share
+inline int mask_splits(const AttnParams& p) { return p.mask ? cdiv(cdiv(p.kv_len, kRows), kMaskTiles) : 1; }
 
 // Every warp packs its share of the mask's bytes for the key tiles [first, end), as far as there are keys.
 __device__ __forceinline__ void pack_key_bits(uint32_t* words, const unsigned char* mask, int first, int end, int len,
