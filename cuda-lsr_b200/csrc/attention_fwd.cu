@@ -476,8 +476,9 @@ int query_tiles(const AttnParams& p) {
 // the SMs have room for, with four tiles each at least, so that the join does not cost more than it saves. And as many
 // as a long mask's bits take.
 int split_count(const AttnParams& p) {
-  const long long blocks = (long long)cdiv(p.q_len, query_tiles(p) * kRows) * p.heads * p.batch;
-  const int tiles = cdiv(p.kv_len, kRows), room = 2 * device_sm_count();
+  const int pair = query_tiles(p), room = (pair == 2 ? 1 : 2) * device_sm_count();
+  const long long blocks = (long long)cdiv(p.q_len, pair * kRows) * p.heads * p.batch;
+  const int tiles = cdiv(p.kv_len, kRows);
   return (int)std::max<long long>(mask_splits(p), std::min<long long>(std::min<long long>(room / blocks, tiles / 4), 64));
 }
 

@@ -95,3 +95,14 @@ def test_entries_of_a_batch_more_than_2_31_apart(dtype):
         r += A.attention_forward(*ts, causal=True)
         r += A.attention_backward(do, *ts, *r, causal=True)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("more", [0, 1])
+def test_a_grid_that_fills_the_gpu_is_not_split(more):
+    """A block of two query tiles has an SM to itself: with one for each SM, keys dealt to two would only queue."""
+    from lsr import _lib
+    from lsr import attention as A
+    h = torch.cuda.get_device_properties(0).multi_processor_count + more
+    q, k = (torch.zeros(1, n, h, 64, device="cuda", dtype=torch.bfloat16) for n in (256, 1024))
+    out, lse = A.attention_forward(q, k, k)
+    assert _lib.load().lsr_attention_forward_workspace_bytes(A._pack(q, k, k, None, False, None, out, lse)) == 0
