@@ -28,6 +28,7 @@ constexpr int GR_TABLE = 1024;     // tensors per launch at most (30 bytes each 
 constexpr int GR_SMALL = 96;       // a shorter list takes kernels with 3 KB of parameters instead of 30: less to copy per launch
 constexpr int GR_CLUSTER = 8;      // blocks that take a short list in one launch
 constexpr int GR_SHORT = 64;       // chunks of a short list
+static_assert(GR_SHORT <= GR_SMALL, "a tensor has a chunk at least: only small tables hold short lists");
 constexpr int GR_GRID = 592;       // blocks: 148 SMs x 4 blocks of 512 threads
 enum : int { NORM_MAX = 0, NORM_ONE = 1, NORM_TWO = 2 };
 
@@ -327,8 +328,9 @@ void fill_table(GradTable<N>& t, const void* const* in, void* const* out, const 
                 const int* tout, int n, int* i) {
   t.n = 0;
   t.chunks = 0;
-  for (; *i < n && t.n < N; ++*i) {
+  for (; *i < n; ++*i) {
     if (!numel[*i]) continue;
+    if (t.n == N) break;
     const long long c = (numel[*i] + GR_CHUNK - 1) / GR_CHUNK;
     if (t.n && t.chunks + c > (1ll << 30)) break;
     t.in[t.n] = in[*i];
@@ -367,12 +369,13 @@ int norm_table(const void* const* in, const long long* numel, const int* tin, in
               cudaStream_t st) {
   GradTable<N> t;
   int taken = 0;
-  fill_table(t, in, nullptr, numel, tin, nullptr, n, &taken);
-  if (taken == n && t.chunks <= GR_SHORT) {
-    ProfScope prof(PK_EW_OTHER, st);
-    grad_short_kernel<KIND, false, N><<<GR_CLUSTER, GR_THREADS, 0, st>>>(t, 0.f, norm);
-    return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
-  }
+  if constexpr (N == GR_SMALL) fill_table(t, in, nullptr, numel, tin, nullptr, n, &taken);
+  if constexpr (N == GR_SMALL)
+    if (taken == n && t.chunks <= GR_SHORT) {
+      ProfScope prof(PK_EW_OTHER, st);
+      grad_short_kernel<KIND, false, N><<<GR_CLUSTER, GR_THREADS, 0, st>>>(t, 0.f, norm);
+      return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
+    }
   auto* partial = static_cast<Acc<KIND>*>(ws);
   int count = 0;
   const int rc = launch_partials<KIND, N>(t, in, numel, tin, n, partial, (int)(bytes / sizeof(double)), &count, st);
@@ -389,12 +392,14 @@ int clip_table(const void* const* in, void* const* out, const long long* numel, 
   auto* partial = static_cast<Acc<KIND>*>(ws);
   int count = 0;
   if (!GIVEN) {
-    int taken = 0;
-    fill_table(t, in, out, numel, tin, tout, n, &taken);
-    if (taken == n && t.chunks <= GR_SHORT) {
-      ProfScope prof(PK_EW_OTHER, st);
-      grad_short_kernel<KIND, true, N><<<GR_CLUSTER, GR_THREADS, 0, st>>>(t, max_norm, norm);
-      return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
+    if constexpr (N == GR_SMALL) {
+      int taken = 0;
+      fill_table(t, in, out, numel, tin, tout, n, &taken);
+      if (taken == n && t.chunks <= GR_SHORT) {
+        ProfScope prof(PK_EW_OTHER, st);
+        grad_short_kernel<KIND, true, N><<<GR_CLUSTER, GR_THREADS, 0, st>>>(t, max_norm, norm);
+        return cudaGetLastError() == cudaSuccess ? LSR_OK : LSR_ERR_LAUNCH;
+      }
     }
     const int rc = launch_partials<KIND, N>(t, in, numel, tin, n, partial, (int)(bytes / sizeof(double)), &count, st);
     if (rc != LSR_OK) return rc;
@@ -412,17 +417,24 @@ int clip_table(const void* const* in, void* const* out, const long long* numel, 
   return LSR_OK;
 }
 
+// Whether the tensors that have entries fit a small table (with more, no list is a short one).
+bool few(const long long* numel, int n) {
+  int k = 0;
+  for (int i = 0; i < n && k <= GR_SMALL; ++i) k += numel[i] > 0;
+  return k <= GR_SMALL;
+}
+
 template <int KIND>
 int norm_impl(const void* const* in, const long long* numel, const int* tin, int n, float* norm, void* ws, size_t bytes,
               cudaStream_t st) {
-  return n <= GR_SMALL ? norm_table<KIND, GR_SMALL>(in, numel, tin, n, norm, ws, bytes, st)
+  return few(numel, n) ? norm_table<KIND, GR_SMALL>(in, numel, tin, n, norm, ws, bytes, st)
                        : norm_table<KIND, GR_TABLE>(in, numel, tin, n, norm, ws, bytes, st);
 }
 
 template <int KIND, bool GIVEN>
 int clip_impl(const void* const* in, void* const* out, const long long* numel, const int* tin, const int* tout, int n,
               float max_norm, float* norm, void* ws, size_t bytes, cudaStream_t st) {
-  return n <= GR_SMALL
+  return few(numel, n)
              ? clip_table<KIND, GIVEN, GR_SMALL>(in, out, numel, tin, tout, n, max_norm, norm, ws, bytes, st)
              : clip_table<KIND, GIVEN, GR_TABLE>(in, out, numel, tin, tout, n, max_norm, norm, ws, bytes, st);
 }

@@ -21,6 +21,8 @@ LISTS = {
     "1024": [(i % 37 + 1,) for i in range(1024)],
     "1025": [(i % 37 + 1,) for i in range(1025)],
     "empty ones among": [(0,) if i % 3 else (i % 91 + 1,) for i in range(3000)],
+    "96 and empty ones": [(i % 37 + 1,) for i in range(96)] + [(0,)] * 50,
+    "50 among empty ones": [(0,) if i % 4 else (3000 * (i % 7) + 1,) for i in range(200)],
     "three tables": [(i % 37 + 1,) for i in range(2500)] + [(300, 1001)],
 }
 
