@@ -19,15 +19,22 @@
 // of the five products; dim 128: 1907 us, 720.
 // P and dS are rounded to 16 bits for the products: half a step of each term, which leaves the gradients with a relative error
 // of 0.0024 in bf16 and 0.0003 in fp16, at 8 keys as at 4096, where the rounding of the results alone makes 0.0017 and
-// 0.0002. A second 16-bit part of dS would bring dq and dk down to that, dv not, for 17.3 us instead of 15.5 at 25
-// heads x 512 x 64. In fp16 P is taken times 2^10 (at most 1024), so
+// 0.0002. In rows of n keys D adds to that: o was rounded, and computed from a rounded P, which makes 2 / n of
+// what dS's rounding does. It is the first rows of a causal sequence that this shows in, at any length, since they
+// make up most of the gradients' size. So blocks of rows with at most kFewKeys keys (query tiles; key tiles that such
+// rows begin at) multiply dS in two parts, the rounded value and what that left. Over a causal training step of 1000
+// tokens dq is then off by 1.24 to 1.41 times what rounding the result alone makes, 1.44 to 1.58 without; it is at
+// most two tiles of a sequence that pay for it.
+// In fp16 P is taken times 2^10 (at most 1024), so
 // that rows over thousands of keys stay above its smallest normal value; dV is scaled back. dS has no size of its own
 // (loss-scaled gradients pass fp16's largest value, small ones over many keys lie among its smallest), so in fp16
 // it is taken times 2^x, one x for a key head and the query heads that share it, from
 //   |dS| <= |dO_i| (max |v_j| + |o_i|) <= B = 2 max |dO_i| max |v_j|,   2^13 <= 2^x B < 2^14,
 // over the rows that are seen and finite: nothing overflows, and what is lost lies 2^-38 below B. The kernel that takes D
-// leaves the largest of each tile, and every block takes the largest of those again (8 x 16 heads x 1024 x 64 causal: 144.7 us,
-// 143.6 without; dS unscaled lost a tenth of dq at dout of 1e-4 on 8192 keys, and made NaN of dP beyond 2^17).
+// leaves the largest of each tile, and every block takes the largest of those again (8 x 16 heads x 1024 x 64 causal: 146.7 us,
+// 141.6 in bf16; dS unscaled lost a tenth of dq at dout of 1e-4 on 8192 keys, and made NaN of dP beyond 2^17).
+#include <type_traits>
+
 #include "attention_sm100.cuh"
 
 namespace lsr {
@@ -39,6 +46,9 @@ constexpr int BWD_THREADS = PARTS * 128 + 128;  // then the loader, the issuer, 
 constexpr int LOADER = 4 * PARTS, ISSUER = LOADER + 1, SIZER = ISSUER + 1;
 // Registers a thread after the split, within the 96 that five warpgroups are launched with: 5 x 96 = 4 x 104 + 64.
 constexpr int kScoreRegs = 104, kRestRegs = 64;
+
+// Of more keys D's part is under 2% of dS's own rounding.
+constexpr int kFewKeys = 128;
 
 // Whether dS is scaled to a size of the data.
 template <typename T>
@@ -59,7 +69,8 @@ struct BwdParams {
   // kSized: the largest |dout row|^2 of each tile, [batch][heads][q_tiles], then the largest |v row|^2 among its keys that are
   // seen, [batch][kv_heads][kv_tiles]; rows that are not finite do not count
   float* sizes;
-  long long size_rows;  // query tiles
+  long long size_rows, size_keys;  // tiles of each
+  int2* seen;                      // [batch] with a mask: the first key that is seen, and how many are
   int q_tiles, kv_tiles;
   long long kv_blocks;
   // blocks that the steps of 128 keys, and of 128 queries, are dealt to; with more than one their sums go here
@@ -94,10 +105,29 @@ __device__ __forceinline__ float row_sum(float s) {
 
 // Row statistics: a tile of 128 rows per block, eight lanes per row, four rows per thread in flight (one row per thread and
 // 32 per block: 23.5 us at 8 x 16 heads x 1024 x 64 in fp16, now 12.8). kSized: the blocks after those of the
-// queries take the sizes of the values.
+// queries take the sizes of the values. The last blocks look the masks over, one each.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ BwdParams p) {
+  __shared__ unsigned tops[8];
   launch_dependents();
+  if (blockIdx.x >= p.size_rows + p.size_keys) {
+    __shared__ unsigned counts[8];
+    const unsigned b = blockIdx.x - (unsigned)(p.size_rows + p.size_keys);
+    const unsigned char* mask = p.a.mask + b * p.a.mask_stride;
+    unsigned first = p.a.kv_len, count = 0;
+#pragma unroll 8
+    for (int j = threadIdx.x; j < p.a.kv_len; j += 256)
+      if (mask[j]) first = min(first, (unsigned)j), ++count;
+    first = __reduce_min_sync(0xffffffffu, first);
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = first, counts[threadIdx.x / 32] = count;
+    __syncthreads();
+    if (threadIdx.x) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) first = min(first, tops[w]), count += counts[w];
+    p.seen[b] = make_int2((int)first, (int)count);
+    return;
+  }
   const bool keys = kSized<T> && blockIdx.x >= p.size_rows;
   const long long id = blockIdx.x - (keys ? p.size_rows : 0);
   const int tiles = keys ? p.kv_tiles : p.q_tiles, heads = keys ? p.a.kv_heads : p.a.heads;
@@ -149,7 +179,6 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
     }
   }
   if (!kSized<T>) return;
-  __shared__ unsigned tops[8];
   unsigned top = 0;  // of the finite ones: values >= 0 are ordered as their bits are
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -178,6 +207,16 @@ __device__ __forceinline__ float ds_scale(const BwdParams& p, int b, int hk, int
                       sqrtf(__uint_as_float(__reduce_max_sync(0xffffffffu, v2)));
   // 2^-47 to 2^41, or 0
   return bound > 0.f ? __uint_as_float((2 * 127 + 13 - (__float_as_uint(bound) >> 23)) << 23) : 1.f;
+}
+
+// Query tiles before this one have rows of few keys, as far as causality and the first key that a mask leaves tell (or none).
+template <bool MASK>
+__device__ __forceinline__ int few_key_tiles(const BwdParams& p, int b) {
+  const int2 seen = MASK ? p.seen[b] : make_int2(0, p.a.kv_len);
+  if (seen.y <= kFewKeys) return 0x7fffffff;
+  // the row that sees kFewKeys keys from that first one on
+  const int last = seen.x + kFewKeys - 1 - (p.a.kv_len - p.a.q_len);
+  return p.a.causal && last >= 0 ? last / kRows + 1 : 0;
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -358,6 +397,8 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
       const uint32_t idesc_t = make_idesc(128, 128, umma_format<T>(), 0, 0);
       const uint32_t idesc_a = make_idesc(128, ksteps * 16, umma_format<T>(), 0, 1);
       const uint32_t ra1 = smem_u32(r1), ra2 = smem_u32(r2), xa = smem_u32(ring);
+      if (MASK) wait_dependency();
+      const bool low = (KEYS ? first : tile) < few_key_tiles<MASK>(p, b);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         ok = ok && warp_wait(bar, parity, abort_flag, status, ST_ATTN_MMA);
@@ -404,6 +445,7 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
         if (!wait(ds_ready, pph)) break;
         if (elect_one()) {
           mma_probs<128, COLS, COLS>(acc2, t2, x1, idesc_a, more);
+          if (low) mma_probs<128, COLS, COLS>(acc2, t2 + COLS / 2, x1, idesc_a, 1);
           umma_commit(left);
           if (jn < steps) scores2();
         }
@@ -443,98 +485,116 @@ __device__ __forceinline__ void bwd_block(const BwdParams& p, unsigned x, uint8_
     int cur = 0;  // stage of the step's first tile
     uint32_t sph = 0;
     float lse = 0.f, delta = 0.f;
+    if (MASK || !KEYS) wait_dependency();
+    const bool low = (KEYS ? first : tile) < few_key_tiles<MASK>(p, b);
     if (!KEYS) {
-      wait_dependency();
       const float* st = p.stats + (((long long)b * p.a.heads + h) * p.q_tiles + tile) * 256 + r;
       lse = st[0] + (float)kExtra<T>;
       delta = st[128];
     }
     if (kSized<T>) ok = warp_wait(sized, 0, abort_flag, status, ST_ATTN_SOFTMAX);
-    for (int j = start; ok && j < steps; j = bits.next(j + 1, steps)) {
-      const int t0 = (KEYS ? first + j % tiles : j) * kRows + part * COLS;  // position of the thread's first column
-      // the statistics come with the step's first tile
-      if (KEYS && !(ok = warp_wait(full + cur, sph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
-      const float4* stat = reinterpret_cast<const float4*>(smem + L::STATS + cur / 2 * 1024) + part * (COLS / 4);
-      if (!(ok = warp_wait(t1_full, ph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
-      tc_fence_after();
-      uint32_t s[COLS];
-      tmem_ld32(my1, s);
-      tmem_ld_wait();
-      uint32_t word = ~0u;  // which of the thread's keys are seen
-      if (MASK && !KEYS) word = reinterpret_cast<const uint32_t*>(bits.bits + j)[part];
-      if (KEYS) {
-        if (p.a.causal && row0 + kRows - 1 > t0 + off) {
-          const int from = row - off - t0;  // queries before it do not see the key
+    auto run = [&](auto parts) {
+      for (int j = start; ok && j < steps; j = bits.next(j + 1, steps)) {
+        const int t0 = (KEYS ? first + j % tiles : j) * kRows + part * COLS;  // position of the thread's first column
+        // the statistics come with the step's first tile
+        if (KEYS && !(ok = warp_wait(full + cur, sph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
+        const float4* stat = reinterpret_cast<const float4*>(smem + L::STATS + cur / 2 * 1024) + part * (COLS / 4);
+        if (!(ok = warp_wait(t1_full, ph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
+        tc_fence_after();
+        uint32_t s[COLS];
+        tmem_ld32(my1, s);
+        tmem_ld_wait();
+        uint32_t word = ~0u;  // which of the thread's keys are seen
+        if (MASK && !KEYS) word = reinterpret_cast<const uint32_t*>(bits.bits + j)[part];
+        if (KEYS) {
+          if (p.a.causal && row0 + kRows - 1 > t0 + off) {
+            const int from = row - off - t0;  // queries before it do not see the key
+#pragma unroll
+            for (int e = 0; e < COLS; ++e)
+              if (e < from) s[e] = 0xff800000u;
+          }
+        } else {
+          warp_arrive(p_ready, lane);  // T1 is in registers
+          const int sees = min(p.a.kv_len, p.a.causal ? row + off + 1 : p.a.kv_len) - t0;
+          if (word != ~0u || t0 + COLS > p.a.kv_len || (p.a.causal && t0 + COLS - 1 > row0 + off)) {
+#pragma unroll
+            for (int e = 0; e < COLS; ++e)
+              if (e >= sees || (MASK && !((word >> e) & 1))) s[e] = 0xff800000u;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < COLS; e += 4) {
+          const float4 v = KEYS ? stat[e / 4] : make_float4(lse, lse, lse, lse);
+          float x[4];
+          unpair(fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, pair(-v.x, -v.y)), x[0], x[1]);
+          unpair(fma2(pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), c2, pair(-v.z, -v.w)), x[2], x[3]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[e + k] = __float_as_uint(ex2(x[k]));
+        }
+        if (KEYS) {
+          uint32_t pr[COLS / 2];
+#pragma unroll
+          for (int e = 0; e < COLS / 2; ++e) pr[e] = pack2<T>(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+          tmem_st16(my1, pr);
+          tmem_st_wait();
+          warp_arrive(p_ready, lane);
+        }
+        if (!(ok = warp_wait(t2_full, ph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
+        tc_fence_after();
+        uint32_t d[COLS], pr[COLS / 2];
+        tmem_ld32(my2, d);
+        tmem_ld_wait();
+        if (word != ~0u) {  // what a hidden key's values hold must not reach 0 times it
 #pragma unroll
           for (int e = 0; e < COLS; ++e)
-            if (e < from) s[e] = 0xff800000u;
+            if (!((word >> e) & 1)) d[e] = 0;
         }
-      } else {
-        warp_arrive(p_ready, lane);  // T1 is in registers
-        const int sees = min(p.a.kv_len, p.a.causal ? row + off + 1 : p.a.kv_len) - t0;
-        if (word != ~0u || t0 + COLS > p.a.kv_len || (p.a.causal && t0 + COLS - 1 > row0 + off)) {
+        // kSized: P times 2^x (read again in every step: there are no registers to spare), and without its extra power
+        const float up = kSized<T> ? *size_slot : 1.f;
+        const uint64_t by = pair(up * (1.f / (1 << (KEYS ? kExtra<T> : 0))), up * (1.f / (1 << (KEYS ? kExtra<T> : 0))));
 #pragma unroll
-          for (int e = 0; e < COLS; ++e)
-            if (e >= sees || (MASK && !((word >> e) & 1))) s[e] = 0xff800000u;
+        for (int e = 0; e < COLS; e += 4) {
+          const float4 v = KEYS ? stat[32 + e / 4] : make_float4(delta, delta, delta, delta);
+          uint64_t p0 = pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+          uint64_t p1 = pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+          if (kSized<T>) p0 = mul2(p0, by), p1 = mul2(p1, by);
+          float x[4];
+          unpair(mul2(add2(pair(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), pair(-v.x, -v.y)), p0), x[0], x[1]);
+          unpair(mul2(add2(pair(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])), pair(-v.z, -v.w)), p1), x[2], x[3]);
+          pr[e / 2] = pack2<T>(x[0], x[1]);
+          pr[e / 2 + 1] = pack2<T>(x[2], x[3]);
+          if (parts.value == 2) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) d[e + k] = __float_as_uint(x[k]);
+          }
         }
-      }
+        tmem_st16(my2, pr);
+        if (parts.value == 2) {  // what the rounding left, beside it
 #pragma unroll
-      for (int e = 0; e < COLS; e += 4) {
-        const float4 v = KEYS ? stat[e / 4] : make_float4(lse, lse, lse, lse);
-        float x[4];
-        unpair(fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, pair(-v.x, -v.y)), x[0], x[1]);
-        unpair(fma2(pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), c2, pair(-v.z, -v.w)), x[2], x[3]);
+          for (int e = 0; e < COLS / 2; ++e) {
+            const float2 hi = unpack2<T>(pr[e]);
+            pr[e] = pack2<T>(__uint_as_float(d[2 * e]) - hi.x, __uint_as_float(d[2 * e + 1]) - hi.y);
+          }
+          tmem_st16(my2 + COLS / 2, pr);
+        }
+        if (MASK && !KEYS) {  // nor what its keys hold
+          const uint32_t seen = reinterpret_cast<const uint32_t*>(bits.bits + j)[r / 32];
+          if (!((seen >> lane) & 1) && part < PANELS) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[e + k] = __float_as_uint(ex2(x[k]));
-      }
-      if (KEYS) {
-        uint32_t pr[COLS / 2];
-#pragma unroll
-        for (int e = 0; e < COLS / 2; ++e) pr[e] = pack2<T>(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
-        tmem_st16(my1, pr);
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(ring + cur * L::TILE + part * kPanel + r * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
         tmem_st_wait();
-        warp_arrive(p_ready, lane);
+        warp_arrive(ds_ready, lane);
+        ph ^= 1;
+        cur += 2;
+        if (cur == STAGES) cur = 0, sph ^= 1;
       }
-      if (!(ok = warp_wait(t2_full, ph, abort_flag, status, ST_ATTN_SOFTMAX))) break;
-      tc_fence_after();
-      uint32_t d[COLS], pr[COLS / 2];
-      tmem_ld32(my2, d);
-      tmem_ld_wait();
-      if (word != ~0u) {  // what a hidden key's values hold must not reach 0 times it
-#pragma unroll
-        for (int e = 0; e < COLS; ++e)
-          if (!((word >> e) & 1)) d[e] = 0;
-      }
-      // kSized: P times 2^x (read again in every step: there are no registers to spare), and without its extra power
-      const float up = kSized<T> ? *size_slot : 1.f;
-      const uint64_t by = pair(up * (1.f / (1 << (KEYS ? kExtra<T> : 0))), up * (1.f / (1 << (KEYS ? kExtra<T> : 0))));
-#pragma unroll
-      for (int e = 0; e < COLS; e += 4) {
-        const float4 v = KEYS ? stat[32 + e / 4] : make_float4(delta, delta, delta, delta);
-        uint64_t p0 = pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), p1 = pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
-        if (kSized<T>) p0 = mul2(p0, by), p1 = mul2(p1, by);
-        float x[4];
-        unpair(mul2(add2(pair(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), pair(-v.x, -v.y)), p0), x[0], x[1]);
-        unpair(mul2(add2(pair(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])), pair(-v.z, -v.w)), p1), x[2], x[3]);
-        pr[e / 2] = pack2<T>(x[0], x[1]);
-        pr[e / 2 + 1] = pack2<T>(x[2], x[3]);
-      }
-      tmem_st16(my2, pr);
-      if (MASK && !KEYS) {  // nor what its keys hold
-        const uint32_t seen = reinterpret_cast<const uint32_t*>(bits.bits + j)[r / 32];
-        if (!((seen >> lane) & 1) && part < PANELS) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<uint4*>(ring + cur * L::TILE + part * kPanel + r * 128 + e * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-      }
-      tmem_st_wait();
-      warp_arrive(ds_ready, lane);
-      ph ^= 1;
-      cur += 2;
-      if (cur == STAGES) cur = 0, sph ^= 1;
-    }
+    };
+    if (low) run(std::integral_constant<int, 2>());  // two bodies: the common one keeps nothing for the second part
+    else run(std::integral_constant<int, 1>());
     if (ok) ok = warp_wait(done, 0, abort_flag, status, ST_ATTN_SOFTMAX);
     tc_fence_after();
     if (ok) {
@@ -614,7 +674,7 @@ int launch(BwdParams& p, cudaStream_t st) {
   using L = BwdSmem<PANELS, MASK>;
   static_assert(L::TOTAL <= 232448, "shared memory budget exceeded");
   const long long blocks = p.kv_blocks + (long long)p.q_tiles * p.a.heads * p.a.batch * p.split_q;
-  const long long stat_blocks = p.size_rows + (kSized<T> ? (long long)p.kv_tiles * p.a.kv_heads * p.a.batch : 0);
+  const long long stat_blocks = p.size_rows + p.size_keys + (MASK ? p.a.batch : 0);
   if (blocks > 0x7fffffffll || stat_blocks > 0x7fffffffll) return LSR_ERR_SHAPE;
   {
     ProfScope prof(PK_EW_OTHER, st);
@@ -669,10 +729,17 @@ int backward(BwdParams& p, cudaStream_t st) {
   return p.a.mask ? launch<T, 1, true>(p, st) : launch<T, 1, false>(p, st);
 }
 
-// Entries of BwdParams::sizes, rounded up so that 16-byte alignment goes on.
-size_t size_count(const BwdParams& p, int dtype) {
-  const size_t n = ((size_t)p.q_tiles * p.a.heads + (size_t)p.kv_tiles * p.a.kv_heads) * p.a.batch;
-  return dtype == LSR_DTYPE_F16 ? (n + 3) / 4 * 4 : 0;
+// Where the workspace's parts begin, each on 16 bytes; the partial sums come last. The floats before those.
+size_t place(BwdParams& p, int dtype, void* ws) {
+  const auto up4 = [](size_t n) { return (n + 3) / 4 * 4; };
+  p.size_rows = (long long)p.q_tiles * p.a.heads * p.a.batch;
+  p.size_keys = dtype == LSR_DTYPE_F16 ? (long long)p.kv_tiles * p.a.kv_heads * p.a.batch : 0;
+  p.stats = static_cast<float*>(ws);
+  const size_t sizes = (size_t)p.size_rows * 256;
+  const size_t seen = sizes + (dtype == LSR_DTYPE_F16 ? up4(p.size_rows + p.size_keys) : 0);
+  p.sizes = p.stats + sizes;
+  p.seen = reinterpret_cast<int2*>(p.stats + seen);
+  return seen + (p.a.mask ? up4(2 * (size_t)p.a.batch) : 0);
 }
 
 }  // namespace
@@ -681,7 +748,7 @@ size_t attention_backward_sm100_ws(const AttnParams& a, int dtype) {
   BwdParams p{};
   p.a = a;
   set_splits(p);
-  size_t floats = (size_t)p.q_tiles * a.heads * a.batch * 256 + size_count(p, dtype);
+  size_t floats = place(p, dtype, nullptr);
   if (p.split_k > 1) floats += (size_t)p.split_k * 2 * a.batch * a.kv_heads * a.kv_len * a.head_dim;
   if (p.split_q > 1) floats += (size_t)p.split_q * a.batch * a.heads * a.q_len * a.head_dim;
   return floats * sizeof(float);
@@ -691,10 +758,7 @@ int attention_backward_sm100(const AttnParams& a, int dtype, void* ws, cudaStrea
   BwdParams p{};
   p.a = a;
   set_splits(p);
-  p.stats = static_cast<float*>(ws);
-  p.size_rows = (long long)p.q_tiles * a.heads * a.batch;
-  p.sizes = p.stats + (size_t)p.q_tiles * a.heads * a.batch * 256;
-  p.part_dk = p.sizes + size_count(p, dtype);
+  p.part_dk = static_cast<float*>(ws) + place(p, dtype, ws);
   const size_t kv = p.split_k > 1 ? (size_t)p.split_k * a.batch * a.kv_heads * a.kv_len * a.head_dim : 0;
   p.part_dv = p.part_dk + kv;
   p.part_dq = p.part_dv + kv;

@@ -123,6 +123,17 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 }
 
 template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+template <typename T>
 constexpr uint32_t umma_format();
 template <>
 constexpr uint32_t umma_format<__nv_bfloat16>() { return 1; }

@@ -474,7 +474,8 @@ LSR_API int lsr_grad_clip(const void* const* grads, void* const* outs, const lon
  * of k and v hold does not matter, NaN included. head_dim 1..128; strides in
  * elements (batch, position, head), the head_dim entries of a head contiguous.
  * Probabilities and sums are fp32; with 16-bit types p and ds are rounded to
- * that type as operands of the products that take them, whatever the lengths. In
+ * that type as operands of the products that take them (ds in two parts in tiles
+ * of 128 queries some of which see at most 128 keys). In
  * fp16 ds is brought to its range by a power of two of the data first: it loses
  * at most 2^-38 of 2 max |dout_i| max |v_j| of its key head beside the rounding,
  * and overflows only where the gradients themselves do.
