@@ -12,7 +12,7 @@
 // What bounds it: per 128 x 128 tile the exponentials take 1024 cycles of the special function units and
 // the products 1024 cycles of the tensor core at dim 128, 512 at dim 64. Measured (bf16, 4 x 16 heads x
 // 4096, no mask): dim 128 464 to 499 us from run to run, 1100 to 1185 TFLOP/s; dim 64 350 to 367 us, 749 to
-// 786 TFLOP/s, where those units are busy 58% of the time. Exponentials by polynomial on the FMA
+// 786 TFLOP/s, where those units take instructions in 75% of the cycles and the tensor core works in 37%. Exponentials by polynomial on the FMA
 // units for one pair in eight made it slower (413 us): issue slots and latency, not the units, are short.
 // O is rescaled only when a row's maximum has grown by more than 2^8 since it last was: until then P is
 // taken against the old maximum, which fp32 sums and 16-bit P (at most 2^8) hold without loss, and O /

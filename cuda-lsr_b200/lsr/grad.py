@@ -4,8 +4,9 @@
 * ``clip_grads(grads, max_norm, norm_type, out, total_norm)``
                                                       scaled by min(1, max_norm / (norm + 1e-6)), in
                                                       place or into ``out`` of another type
-* ``clip_grad_norm_(parameters, max_norm, ...)``      the same on ``p.grad``, as
-                                                      ``torch.nn.utils.clip_grad_norm_`` is called
+* ``clip_grad_norm_(parameters, max_norm, ...)``      the same on ``p.grad``, with the first four arguments
+                                                      of ``torch.nn.utils.clip_grad_norm_`` (norms 1, 2
+                                                      and inf, gradients on one device; no ``foreach``)
 
 The tensors may mix fp32, bf16 and fp16 and any shapes; norms are fp32 device scalars, summed in 64
 bits in one fixed order, and nothing waits for the device unless ``error_if_nonfinite`` is set. Every
