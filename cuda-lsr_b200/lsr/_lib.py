@@ -268,13 +268,21 @@ def require_cuda(t: torch.Tensor, name: str) -> None:
 _requires_grad_of = torch.Tensor.requires_grad.__get__
 
 
-def differentiated(tensors) -> bool:
-    """Whether autograd follows any of `tensors` now, backward or forward."""
-    if torch.is_grad_enabled() and any(map(_requires_grad_of, tensors)):
-        return True
-    # (the level says that no forward-mode pass is on without a look at each tensor)
+def duals(tensors) -> bool:
+    """Whether one of `tensors` is a dual of a forward-mode pass."""
+    # (the level says that there is no such pass without a look at each tensor)
     return (getattr(forward_ad, "_current_level", 0) >= 0
             and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
+
+
+def refuse_duals(what: str, tensors) -> None:
+    if duals(tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
+def differentiated(tensors) -> bool:
+    """Whether autograd follows any of `tensors` now, backward or forward."""
+    return torch.is_grad_enabled() and any(map(_requires_grad_of, tensors)) or duals(tensors)
 
 
 class _NoGradient(torch.autograd.Function):

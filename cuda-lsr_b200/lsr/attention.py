@@ -20,8 +20,8 @@ rounding the exact ones makes (bf16 0.0024 relative, fp16 0.0003). fp32 tensors 
 
 The backward pass computes the probabilities again from lse; memory grows with the lengths, not with
 their product. Same inputs, same bits: nothing is summed in an order that varies. There is no dropout,
-no second derivative and no forward-mode derivative (NotImplementedError); a gradient through the two halves raises
-RuntimeError. A captured backward pass wants no eager graph of the same leaves alive
+no second derivative and no forward-mode derivative (NotImplementedError). The two halves lie outside autograd: what
+they return is cut off from the graph of their inputs. A captured backward pass wants no eager graph of the same leaves alive
 (PyTorch adds to a leaf's gradient on the stream of the leaf's first graph). The reference leaves attention to its models' library
 (muon_lm_ddp.py:752-822); there is no CPU path: CPU tensors raise ``ValueError``.
 """
@@ -122,8 +122,9 @@ def _forward(q, k, v, causal, scale, key_mask):
 
 
 def attention_forward(q, k, v, *, causal: bool = False, scale: float | None = None, key_mask=None):
-    """(out, lse): the attention of q over k and v, and the log-sum-exp of each query's scores; no gradient."""
-    return _lib.no_gradient("attention_forward", lambda: _forward(q, k, v, causal, scale, key_mask), (q, k, v))
+    """(out, lse): the attention of q over k and v, and the log-sum-exp of each query's scores, outside autograd."""
+    _lib.refuse_duals("attention_forward", (q, k, v))
+    return _forward(q, k, v, causal, scale, key_mask)
 
 
 def _backward(dout, q, k, v, out, lse, causal, scale, key_mask):
@@ -147,9 +148,9 @@ def _backward(dout, q, k, v, out, lse, causal, scale, key_mask):
 
 
 def attention_backward(dout, q, k, v, out, lse, *, causal: bool = False, scale: float | None = None, key_mask=None):
-    """(dq, dk, dv) from the output's gradient and what attention_forward returned for the same arguments; no gradient."""
-    return _lib.no_gradient("attention_backward", lambda: _backward(dout, q, k, v, out, lse, causal, scale, key_mask),
-                            (dout, q, k, v, out, lse))
+    """(dq, dk, dv) from the output's gradient and what attention_forward returned for the same arguments, outside autograd."""
+    _lib.refuse_duals("attention_backward", (dout, q, k, v, out, lse))
+    return _backward(dout, q, k, v, out, lse, causal, scale, key_mask)
 
 
 class _Attention(torch.autograd.Function):

@@ -246,8 +246,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
     outs = dst
     if not src:
         return torch.zeros(()) if total_norm is None else total_norm
-    if _lib.differentiated([*src, *dst] if total_norm is None else [*src, *dst, total_norm]):  # (not backward: no_grad)
-        raise NotImplementedError("clip_grads has no forward-mode derivative")
+    _lib.refuse_duals("clip_grads", [*src, *dst] if total_norm is None else [*src, *dst, total_norm])
     first = src[0]
     dev = first.device
     if dst[0].get_device() != first.get_device():
