@@ -152,24 +152,54 @@ def _check_shared(grads, outs, norm, checked) -> None:
     """ValueError where an output shares memory with another, itself, a gradient that it is not, or the norm; `checked`
     are the numbers of the pairs (gradient, output) that the library compares with one another by itself."""
     spans = []  # (first byte, end, written, compared by the library, tensor)
+
+    def add(t, written, compared):
+        at = t.data_ptr()
+        spans.append((at, at + sum(c * n for c, n in _steps(t)) + t.element_size(), written, compared, t))
+
     for i, (g, o) in enumerate(zip(grads, outs)):
         if not o.numel():
             continue
         if i not in checked and _repeats(o):
             raise ValueError("an output's entries share memory (an expanded tensor, say): clip a copy of it")
-        same = g is o or (g.data_ptr() == o.data_ptr() and g.stride() == o.stride() and g.dtype == o.dtype)
-        for t, written in ((o, True),) if same else ((o, True), (g, False)):
-            spans.append((t.data_ptr(), written, i in checked, t))
+        add(o, True, i in checked)
+        if not (g is o or (g.data_ptr() == o.data_ptr() and g.stride() == o.stride() and g.dtype == o.dtype)):
+            add(g, False, i in checked)
     if norm is not None:
-        spans.append((norm.data_ptr(), False, False, norm))
-    spans = sorted(((at, at + sum(c * n for c, n in _steps(t)) + t.element_size(), w, c, t) for at, w, c, t in spans),
-                   key=lambda x: x[0])
+        add(norm, False, False)
+    spans.sort(key=lambda x: x[0])
+    first, end = 0, 0
+    for k in range(len(spans) + 1):  # runs of spans that overlap
+        if k < len(spans) and spans[k][0] < end:
+            end = max(end, spans[k][1])
+            continue
+        if any(_share(x[4], y[4]) for x, y in _meeting(_folded(spans[first:k]))
+               if (x[2] or y[2]) and not (x[3] and y[3])):
+            raise ValueError("an output shares memory with another output, a gradient or the norm: clip into copies")
+        first, end = k, spans[k][1] if k < len(spans) else 0
+
+
+def _folded(spans):
+    """The spans, or where all are slices of rows equally far apart, their places within a row: slices that lie side by
+    side then do not meet."""
+    steps = [_steps(x[4]) for x in spans]
+    rows = {max(s)[0] if s else 0 for s in steps}
+    if len(rows) != 1 or 0 in rows:
+        return spans
+    row = rows.pop()
+    at = [(x[0] - spans[0][0]) % row for x in spans]
+    ends = [a + sum(c * n for c, n in s if c != row) + x[4].element_size() for a, s, x in zip(at, steps, spans)]
+    if max(ends) > row:
+        return spans
+    return sorted(((a, e, *x[2:]) for a, e, x in zip(at, ends, spans)), key=lambda x: x[0])
+
+
+def _meeting(spans):
+    """The pairs of them that overlap; in order of their first bytes."""
     open_ = []
     for x in spans:
         open_ = [y for y in open_ if y[1] > x[0]]
-        for y in open_:
-            if (x[2] or y[2]) and not (x[3] and y[3]) and _share(x[4], y[4]):
-                raise ValueError("an output shares memory with another output, a gradient or the norm: clip into copies")
+        yield from ((x, y) for y in open_)
         open_.append(x)
 
 

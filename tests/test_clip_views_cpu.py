@@ -67,3 +67,42 @@ def test_lists_with_strided_outputs():
         flat([b[:, :5]], [b[:, :5]], b.view(-1)[24:25])
     src, dst, back = flat([b[:, :5], c, b[:, 5:]], [b[:, :5], c, b[:, 5:]], b.new_zeros(()))
     assert src[1] is c and dst[1] is c and [o.data_ptr() for o, _ in back] == [b.data_ptr(), b[:, 5:].data_ptr()]
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_lists_against_every_byte(seed):
+    from lsr import grad as G
+    rng, buf = random.Random(100 + seed), torch.zeros(4000)
+    for _ in range(150):
+        if rng.random() < 0.5:  # slices of rows, most of them side by side
+            w, at, ts = buf[:rng.randint(2, 9) * 40].view(-1, 40), 0, []
+            while at < 36:
+                n = rng.randint(1, 9)
+                a = at if rng.random() < 0.95 else max(0, at - 1)
+                ts.append(w[rng.randint(0, 1):, a:min(40, at + n)])
+                at += n
+            rng.shuffle(ts)
+        else:
+            ts = [view(rng, buf[rng.randint(0, 3000):][:300]) for _ in range(rng.randint(1, 4))]
+        seen, want = set(), False
+        for t in ts:
+            p = places(t)
+            want |= len(set(p)) < len(p) or not seen.isdisjoint(p)
+            seen |= set(p)
+        norm = buf[rng.randint(0, 3999):][:1] if rng.random() < 0.3 else None
+        want |= norm is not None and not seen.isdisjoint(places(norm))
+        try:
+            G._check_shared(ts, ts, norm, set())
+            got = False
+        except ValueError:
+            got = True
+        assert got == want, [(t.shape, t.stride(), t.storage_offset()) for t in ts]
+
+
+def test_a_matrix_cut_into_many_columns_is_looked_over_quickly():
+    import time
+    from lsr import grad as G
+    cut = list(torch.zeros(64, 64 * 256).split(64, 1))
+    t = time.perf_counter()
+    G._check_shared(cut, cut, None, set())
+    assert time.perf_counter() - t < 0.1  # 4 ms; 320 where every pair is compared
