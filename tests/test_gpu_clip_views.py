@@ -28,7 +28,7 @@ APART = {
     "columns": lambda b: [b[:, :5], b[:, 5:]],
     "rows": lambda b: [b[::2], b[1::2]],
     "transposed": lambda b: [b.t()[:5], b.t()[5:]],
-    "checkers": lambda b: [b[::2, ::2], b[::2, 1::2], b[1::2, ::2], b[1::2, 1::2]],
+    "every second row and column": lambda b: [b[::2, ::2], b[::2, 1::2], b[1::2, ::2], b[1::2, 1::2]],
     "a row and the rest": lambda b: [b[0], b[1:, 2:], b[1:, :2]],
     "other strides": lambda b: [b.view(-1)[::3], b.view(-1)[1::6]],
     "in itself apart": lambda b: [b.as_strided((2, 2), (3, 2))],
