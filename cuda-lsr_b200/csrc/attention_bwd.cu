@@ -15,8 +15,8 @@
 // next are issued as their operands get ready: while the threads take the exponentials of T1, the
 // tensor core adds dS and computes the next T2; while they form dS, it adds P and computes the next T1.
 // Sixteen warps share a tile's scores, 32 columns a thread: with eight the waits on TMEM and on the special
-// function units showed more (1267 us to 1170 when changed). 4 x 16 heads x 4096 x 64, no mask: 1134 us, 606 TFLOP/s
-// of the five products; dim 128: 1907 us, 720.
+// function units showed more (1267 us to 1170 when changed). 4 x 16 heads x 4096 x 64, no mask: 1130 us, 608 TFLOP/s
+// of the five products; dim 128: 1918 us, 716.
 // P and dS are rounded to 16 bits for the products: half a step of each term, which leaves the gradients with a relative error
 // of 0.0024 in bf16 and 0.0003 in fp16, at 8 keys as at 4096, where the rounding of the results alone makes 0.0017 and
 // 0.0002. In rows of n keys D adds to that: o was rounded, and computed from a rounded P, which makes 2 / n of
@@ -25,14 +25,14 @@
 // rows begin at) multiply dS in two parts, the rounded value and what that left. Over a causal training step of 1000
 // tokens dq is then off by 1.24 to 1.41 times what rounding the result alone makes, 1.44 to 1.58 without; it is at
 // most two tiles of a sequence that pay for it.
-// In fp16 P is taken times 2^10 (at most 1024), so
-// that rows over thousands of keys stay above its smallest normal value; dV is scaled back. dS has no size of its own
+// In fp16 P is taken times 2^10 (at most 1024), so that rows over thousands of keys stay above its smallest normal
+// value; dV is scaled back. dS has no size of its own
 // (loss-scaled gradients pass fp16's largest value, small ones over many keys lie among its smallest), so in fp16
 // it is taken times 2^x, one x for a key head and the query heads that share it, from
 //   |dS| <= |dO_i| (max |v_j| + |o_i|) <= B = 2 max |dO_i| max |v_j|,   2^13 <= 2^x B < 2^14,
 // over the rows that are seen and finite: nothing overflows, and what is lost lies 2^-38 below B. The kernel that takes D
 // leaves the largest of each tile, and every block takes the largest of those again (8 x 16 heads x 1024 x 64 causal: 146.7 us,
-// 141.6 in bf16; dS unscaled lost a tenth of dq at dout of 1e-4 on 8192 keys, and made NaN of dP beyond 2^17).
+// 141.6 in bf16; dS unscaled lost a tenth of dq at dout of 1e-4 on 8192 keys, and overflowed beyond 65504).
 #include <type_traits>
 
 #include "attention_sm100.cuh"
